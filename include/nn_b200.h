@@ -275,8 +275,125 @@ nnb_status nnb_attention_decode(nnb_engine* e, const float* d_qkv, void* d_kcach
                                 const void* d_kpre, const void* d_vpre, size_t pre_len, size_t pre_alloc, size_t group,
                                 const float* d_rope_cos, const float* d_rope_sin, const int* d_pos, size_t n_seq,
                                 size_t n_head, size_t dk, int exact, float* d_out, int8_t* d_q8, float* d_s, int32_t* d_qsum);
-/* synchronises and reports NNB_ERR_TIMEOUT if a kernel gave up on a bounded device-side wait */
+/* synchronises and reports NNB_ERR_TIMEOUT if a kernel gave up on a bounded device-side wait, NNB_ERR_INVALID if one of
+ * the paged-cache operators met a page id, length or position that it could not use (the message says which) */
 nnb_status nnb_engine_check(nnb_engine* e);
+
+/* ================= paged key-value cache: serving ragged batches ==========
+ * nnb_attention_decode keeps one contiguous cache per sequence and one position for all of them.  The operators below
+ * serve sequences of different lengths from a pool of pages: a sequence's position t lies in slot t % page_size of page
+ * d_table[t / page_size].  No counterpart in the reference.
+ *
+ * nnb_paged_cache: the pool of one layer.  d_k, d_v (n_pages, n_head_kv, page_size, pitch) of dtype (NNB_F32 or NNB_BF16),
+ * 16-byte aligned, with pitch = nnb_paged_pitch(dk): dk rounded up to 8 features, the pad features zero (nnb_paged_append
+ * writes them).  dk is even and at most 256; page_size is any number of positions.  d_weight
+ * (n_pages, n_head_kv, page_size) f32, or NULL: the attention that every cached position has received so far, per KV head.
+ *
+ * nnb_paged_seqs: the sequences of a call.  Row s of d_table (table_stride entries apart, max_pages used) lists the pages of
+ * sequence s in order, d_len[s] >= 0 is the number of its cached positions; entries behind the last used page are not read.
+ * Pages may be listed by several sequences (a shared prompt) as long as nothing writes to them.  max_pages * page_size must
+ * be at most 2^30.  n_seq may be 0.
+ *
+ * What lies on the device is checked there: a page id outside the pool, a length outside [0, max_pages * page_size] and a
+ * position outside the rotary tables are skipped or clamped as each operator says, never followed, and reported by the next
+ * nnb_engine_check.  The operators run on the engine's stream, allocate nothing and can be captured; concurrent calls need
+ * workspaces of their own. */
+typedef struct nnb_paged_cache {
+    void* d_k;
+    void* d_v;
+    float* d_weight;
+    int32_t dtype; /* nnb_dtype of keys and values */
+    int32_t n_pages, page_size, n_head_kv, dk;
+} nnb_paged_cache;
+typedef struct nnb_paged_seqs {
+    const int32_t* d_table;
+    const int32_t* d_len;
+    int32_t n_seq, max_pages;
+    size_t table_stride;
+} nnb_paged_seqs;
+/* dk rounded up to 8 */
+size_t nnb_paged_pitch(size_t dk);
+/* index of the row (of pitch elements in d_k / d_v, of one float in d_weight) of position pos of one sequence, whose page
+ * ids h_table_row (max_pages) are host memory; -1 if the position has no page in the pool */
+int64_t nnb_paged_row(const nnb_paged_cache* c, const int32_t* h_table_row, int32_t max_pages, int32_t head, int64_t pos);
+
+/* New tokens for the cache, token-major: row r of d_q holds n_head * dk features, of d_k and d_v n_head_kv * dk, rows
+ * *_stride elements apart (the three may be views of one q|k|v product), all of dtype.
+ * d_row_start (n_seq + 1, ascending): rows d_row_start[s] .. d_row_start[s+1] - 1 are the new tokens of sequence s, in order;
+ * rows outside all of them are left alone.  NULL: one token per sequence, n_rows = n_seq.
+ * d_pos (n_rows): the rotary position of every row; NULL: the position's place in the cache (they differ after an eviction).
+ * With one token per sequence a negative d_pos marks an idle sequence, which is skipped.
+ * d_rope_cos / d_rope_sin (rope_ctx, dk/2) as nnb_rope_tables fills them, or both NULL: no rotation.
+ * d_q_out: the rotated queries, rows q_out_stride apart, or NULL (with d_q NULL and n_head 0: keys and values only); may be
+ * d_q with the same stride. */
+typedef struct nnb_paged_tokens {
+    const void *d_q, *d_k, *d_v;
+    void* d_q_out;
+    size_t q_stride, k_stride, v_stride, q_out_stride;
+    int32_t dtype, n_head;
+    size_t n_rows;
+    const int32_t* d_row_start;
+    const int32_t* d_pos;
+    const float *d_rope_cos, *d_rope_sin;
+    int32_t rope_ctx;
+} nnb_paged_tokens;
+/* Rotates the new tokens' queries and keys (in f32, rounded once to the type they are stored in), writes keys and values
+ * behind the d_len[s] cached positions of their sequence, sets the new positions' weight to 0 and
+ * d_len_out[s] = min(d_len[s] + new tokens, max_pages * page_size) (d_len_out may be NULL, or d_len itself).
+ * A token without a place (behind the table's end, or on a page outside the pool) or with a position outside the tables is
+ * not written. */
+nnb_status nnb_paged_append(nnb_engine* e, const nnb_paged_cache* c, const nnb_paged_seqs* s, const nnb_paged_tokens* t,
+                            int32_t* d_len_out);
+/* Attention of one new token per sequence over its d_len[s] cached positions (append first): for query head h of sequence s,
+ * x_t = scale * q . K_t, d_out = sum_t softmax(x)_t V_t, d_lse = log sum_t exp(x_t), KV head h / (n_head / n_head_kv).
+ * d_q (n_seq, n_head, dk) with sequences q_stride elements apart and d_out (n_seq, n_head, dk) are of dtype; d_lse
+ * (n_seq, n_head) f32 may be NULL.  scale = 0 stands for 1 / sqrt(dk).  A sequence without any position gets d_out = 0 and
+ * d_lse = -inf; positions on a page outside the pool take no part.
+ * accumulate != 0: also adds sum over the group's query heads of softmax(x)_t to the d_weight of every position.
+ * Products and sums are held in f32 (bf16 operands enter exactly); d_ws is device memory of at least
+ * nnb_paged_attention_workspace bytes, 16-byte aligned, whose content need not be kept (0 from that call: invalid
+ * arguments). */
+size_t nnb_paged_attention_workspace(nnb_engine* e, const nnb_paged_cache* c, const nnb_paged_seqs* s, size_t n_head, int accumulate);
+nnb_status nnb_paged_attention_decode(nnb_engine* e, const nnb_paged_cache* c, const nnb_paged_seqs* s, const void* d_q, int dtype,
+                                      size_t q_stride, size_t n_head, float scale, void* d_out, float* d_lse, int accumulate, void* d_ws,
+                                      size_t ws_bytes);
+/* Brings every sequence down to at most `budget` positions, per KV head: kept are the first `sinks` and the last `recent`
+ * positions and, of those between, the budget - sinks - recent that have the largest d_weight (ties: the lower position; a
+ * NaN counts as less than every number).  The kept rows are copied, in order of position, to slots 0.. of the pages that row
+ * s of d_dst_table lists in dst (another pool or the same one; keys, values and weights), and
+ * d_len_out[s] = min(d_len[s], budget).  A sequence within the budget is copied whole.  The source is only read: pages shared
+ * with other sequences stay valid, so the destination's pages must not be listed in s->d_table.  src and dst agree in dtype,
+ * n_head_kv and dk and both have weights; page sizes may differ.  Positions on a source page outside the pool count as
+ * weight 0 and their rows as zero; a row whose destination page is outside the pool is not written.
+ * d_ws as above, of nnb_paged_evict_workspace bytes. */
+size_t nnb_paged_evict_workspace(nnb_engine* e, const nnb_paged_cache* src, const nnb_paged_seqs* s, size_t budget);
+nnb_status nnb_paged_evict(nnb_engine* e, const nnb_paged_cache* src, const nnb_paged_seqs* s, size_t budget, size_t sinks, size_t recent,
+                           const nnb_paged_cache* dst, const int32_t* d_dst_table, size_t dst_max_pages, size_t dst_table_stride,
+                           int32_t* d_len_out, void* d_ws, size_t ws_bytes);
+
+/* Adjusts a batch of logits before sampling: the history-dependent part of the rollout's sampler (nnb_sampling_config) as an
+ * operator of its own, with one setting per sequence.  For token id i of sequence s, in this order (f32, rounded once to
+ * the output's type):
+ *   x += d_bias[i];
+ *   if i is among the last repeat_window (0 = all) of the d_history_len[s] ids of d_history: x = x > 0 ? x / r : x * r;
+ *   if i occurs c > 0 times among those from index d_prompt_len[s] on:      x -= d_frequency[s] * c + d_presence[s];
+ *   if bit i % 32 of word i / 32 of d_allowed is 0:                         x = -inf.
+ * Every pointer except d_logits / d_out may be NULL (that part is off; d_prompt_len NULL = 0).  r = d_repeat[s] <= 0 or 1 is
+ * off.  Ids outside [0, vocab) are ignored (padding), lengths are clamped to [0, max_history].  Rows are the given strides
+ * apart (elements, words; a stride of 0 for d_bias / d_allowed shares one row).  d_out may be d_logits with its stride. */
+typedef struct nnb_logits_config {
+    const int32_t* d_history;
+    size_t history_stride, max_history;
+    const int32_t *d_history_len, *d_prompt_len;
+    int32_t repeat_window;
+    const float *d_repeat, *d_presence, *d_frequency;
+    const float* d_bias;
+    size_t bias_stride;
+    const uint32_t* d_allowed;
+    size_t allowed_stride;
+} nnb_logits_config;
+nnb_status nnb_adjust_logits(nnb_engine* e, const void* d_logits, int dtype, size_t n_seq, size_t vocab, size_t stride,
+                             const nnb_logits_config* cfg, void* d_out, size_t out_stride);
 
 /* Host-buffer convenience: quantise h_x (t,k) f32, run the linear, return h_y (t,out) f32.
  * Copies host->device and device->host inside the call and synchronises. */

@@ -99,6 +99,14 @@ _SIGNATURES = {
     "nnb_attention_fwd": (_I, [_P, _P, _P, _P, _SZ, _SZ, _SZ, _SZ, _I, _P, _P]),
     "nnb_attention_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _SZ, _I, _P, _P, _P, _P]),
     "nnb_attention_decode": (_I, [_P, _P, _P, _P, _SZ, _P, _P, _SZ, _SZ, _SZ, _P, _P, _P, _SZ, _SZ, _SZ, _I, _P, _P, _P, _P]),
+    "nnb_paged_pitch": (_SZ, [_SZ]),
+    "nnb_paged_row": (C.c_int64, [_P, _P, C.c_int32, C.c_int32, C.c_int64]),
+    "nnb_paged_append": (_I, [_P, _P, _P, _P, _P]),
+    "nnb_paged_attention_workspace": (_SZ, [_P, _P, _P, _SZ, _I]),
+    "nnb_paged_attention_decode": (_I, [_P, _P, _P, _P, _I, _SZ, _SZ, C.c_float, _P, _P, _I, _P, _SZ]),
+    "nnb_paged_evict_workspace": (_SZ, [_P, _P, _P, _SZ]),
+    "nnb_paged_evict": (_I, [_P, _P, _P, _SZ, _SZ, _SZ, _P, _P, _SZ, _SZ, _P, _P, _SZ]),
+    "nnb_adjust_logits": (_I, [_P, _P, _I, _SZ, _SZ, _SZ, _P, _P, _SZ]),
     "nnb_attention_rope_fwd": (_I, [_P, _P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _SZ, _I, _P, _P]),
     "nnb_attention_rope_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _SZ, _I, _P, _P, _P, _P]),
     "nnb_bitlinear_fwd_host": (_I, [_P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _P]),

@@ -288,7 +288,8 @@ nnb_status nnb_attention_decode(nnb_engine* e, const float* d_qkv, void* d_kcach
 nnb_status nnb_engine_check(nnb_engine* e)
 {
     NNB_REQUIRE(e, "engine is NULL");
-    return tc_check_errors(e);
+    NNB_TRY(tc_check_errors(e));
+    return paged_check_errors(e);
 }
 
 nnb_status nnb_bitlinear_fwd_host(nnb_engine* e, const uint32_t* d_wq, const float* d_tau,

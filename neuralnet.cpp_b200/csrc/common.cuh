@@ -66,7 +66,8 @@ struct nnb_engine {
     size_t pinned_bytes = 0;
     // counts kernel launches issued through this engine (reported by the benchmark)
     unsigned long long launches = 0;
-    int* dev_flags = nullptr;  // small device block: [0] error flag raised by bounded device-side waits
+    int* dev_flags = nullptr;  // small device block: [0] error flag raised by bounded device-side waits,
+                               // [1] what the paged-cache operators could not use (paged.cuh)
     // partial products of the weight-gradient GEMM when it splits the token axis (allocated at first use)
     float* dw_part = nullptr;
     size_t dw_part_floats = 0;
@@ -301,6 +302,7 @@ nnb_status launch_tc_lmhead_bwd(nnb_engine* e, const int8_t* q, const int8_t* w8
                                 const int32_t* actions, const float* lse, const float* ent, const float* up_lp, const float* up_ent,
                                 size_t t, size_t k, size_t v, float* scratch, __nv_bfloat16* dyb, float* db);
 nnb_status tc_check_errors(nnb_engine* e);
+nnb_status paged_check_errors(nnb_engine* e);  // paged.cu
 nnb_status tc_set_forward_tile(int bn);
 nnb_status launch_expand_weights(nnb_engine* e, const uint32_t* wq, size_t rows, size_t k, int8_t* w8, __nv_bfloat16* wb);
 nnb_status launch_scale_to_bf16(nnb_engine* e, const float* dy, const float* tau, size_t t, size_t out, __nv_bfloat16* dyb);
