@@ -12,6 +12,7 @@ nnb_status paged_check_cache(const char* who, const nnb_paged_cache* c, PagedVie
     NNB_REQUIRE(c->dtype == NNB_F32 || c->dtype == NNB_BF16, "%s: cache dtype %d is neither f32 nor bf16", who, c->dtype);
     NNB_REQUIRE(c->n_pages > 0 && c->page_size > 0 && c->n_head_kv > 0, "%s: the cache has no pages, positions or heads", who);
     NNB_REQUIRE(c->dk > 0 && c->dk <= 256 && c->dk % 2 == 0, "%s: head size %d is not an even number up to 256", who, c->dk);
+    NNB_REQUIRE((long long)c->n_pages * c->page_size <= INT32_MAX / c->n_head_kv, "%s: the pool has more than 2^31 - 1 rows", who);
     NNB_REQUIRE(((uintptr_t)c->d_k | (uintptr_t)c->d_v) % 16 == 0 && (uintptr_t)c->d_weight % 4 == 0,
                 "%s: keys and values must be 16-byte aligned", who);
     *out = PagedView{c->d_k, c->d_v, c->d_weight, c->n_pages, c->page_size, c->n_head_kv, c->dk, (int)nnb_paged_pitch((size_t)c->dk)};

@@ -57,8 +57,8 @@ def _check_decode(cache, table, lens, q, out, lse, scale=None, w_before=None):
     hk, dk, heads = cache.n_head_kv, cache.dk, q.shape[1]
     g = heads // hk
     scale = dk ** -0.5 if scale is None else scale
+    half = HALF[out.dtype]
     out, lse, q = out.cpu().double(), lse.cpu().double(), q.cpu().double()
-    half = HALF[BF16 if out.dtype is None else _check_decode.dtype]
     for i, n in enumerate(lens):
         if n == 0:
             assert bool((out[i] == 0).all()) and bool((lse[i] == -np.inf).all())
@@ -88,7 +88,6 @@ def _decode(pkg, eng, lens, heads, hk, page, dk, cache_dtype, io, seed=0, scale=
     before = [_read(cache, table, i, n)[2] for i, n in enumerate(lens)] if track else None
     out, lse = eng.paged_attention_decode(cache, table, lengths, q, scale=scale or 0.0, accumulate=track)
     eng.check_device_errors()
-    _check_decode.dtype = io
     _check_decode(cache, table, lens, q, out, lse, scale, before)
     return cache, table, lengths, q, out, lse
 
@@ -121,7 +120,6 @@ def test_decode_accumulates_the_attention_weights(pkg, eng, heads, hk, page, dk,
     assert int((~torch.isnan(cache.weight)).sum()) == total
     seen = [_read(cache, table, i, n)[2] for i, n in enumerate(lens)]
     out, lse = eng.paged_attention_decode(cache, table, lengths, q, accumulate=True)  # and once more on top
-    _check_decode.dtype = io
     _check_decode(cache, table, lens, q, out, lse, None, seen)
 
 
@@ -158,7 +156,6 @@ def test_decode_is_the_same_every_time_and_ignores_batch_neighbours(pkg, eng):
     for _ in range(3):
         o, z = eng.paged_attention_decode(cache, table, lengths, q)
         assert torch.equal(o, out) and torch.equal(z, lse)
-    _check_decode.dtype = F32
     o, z = eng.paged_attention_decode(cache, table[2:3], lengths[2:3], q[2:3])
     _check_decode(cache, table[2:3], [2500], q[2:3], o, z)
 
@@ -170,7 +167,6 @@ def test_sequences_may_share_pages(pkg, eng):
     shared[1:, :8] = table[0, :8]
     o, z = eng.paged_attention_decode(cache, shared, lengths, q)
     eng.check_device_errors()
-    _check_decode.dtype = F32
     _check_decode(cache, shared, [256, 300, 280], q, o, z)
 
 
@@ -746,7 +742,6 @@ def test_an_engine_on_its_own_stream_is_ordered_with_torchs(pkg):
         torch.cuda.synchronize()
         want = got if want is None else want
         assert torch.equal(got, want)
-    _check_decode.dtype = F32
     out, lse = e.paged_attention_decode(cache, table, lengths, q)
     _check_decode(cache, table, [600, 30], q, out, lse)
     e.close()
