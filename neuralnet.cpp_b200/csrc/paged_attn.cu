@@ -17,107 +17,19 @@ struct DecodeArgs {
 
 __device__ __forceinline__ float2 load_pair(const float* p) { return make_float2(p[0], p[1]); }
 __device__ __forceinline__ float2 load_pair(const __nv_bfloat16* p) { return make_float2(__bfloat162float(p[0]), __bfloat162float(p[1])); }
+__device__ __forceinline__ float load_one(const float* p) { return *p; }
+__device__ __forceinline__ float load_one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void store_one(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_one(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-// One CTA per (sequence, query head), its four warps on every fourth position each; a lane holds pairs of features.
-template <typename TQ, typename TC>
-__global__ void __launch_bounds__(128) paged_decode_kernel(const PagedView c, const SeqView s, const DecodeArgs a, float* __restrict__ lse_out, int* flags)
-{
-    __shared__ float part[4][258];
-    const int seq = blockIdx.x / a.n_head, h = blockIdx.x % a.n_head, hk = h / a.group;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n = paged_len(c, s, seq, flags);
-    const TQ* q = (const TQ*)a.q + (long long)seq * a.q_stride + (long long)h * c.dk;
-    float2 qf[4], o[4];
-    for (int i = 0; i < 4; ++i) {
-        const int f = 2 * lane + 64 * i;
-        qf[i] = f < c.dk ? load_pair(q + f) : make_float2(0.0f, 0.0f);
-        o[i] = make_float2(0.0f, 0.0f);
-    }
-    float m = -INFINITY, l = 0.0f;
-    for (int t = warp; t < n; t += 4) {
-        const long long row = paged_row(s.table[(long long)seq * s.stride + t / c.page], c.n_pages, c.heads, c.page, hk, t % c.page);
-        if (row < 0) {
-            if (lane == 0) paged_flag(flags, PAGED_BAD_PAGE);
-            continue;
-        }
-        const TC* k = (const TC*)c.k + row * c.pitch;
-        const TC* v = (const TC*)c.v + row * c.pitch;
-        float x = 0.0f;
-        for (int i = 0; i < 4; ++i)
-            if (2 * lane + 64 * i < c.dk) {
-                const float2 kf = load_pair(k + 2 * lane + 64 * i);
-                x = fmaf(qf[i].x, kf.x, fmaf(qf[i].y, kf.y, x));
-            }
-        x = warp_sum(x) * a.scale;
-        const float top = fmaxf(m, x), base = top == -INFINITY ? 0.0f : top;
-        const float old = expf(m - base), p = expf(x - base);
-        l = fmaf(l, old, p);
-        for (int i = 0; i < 4; ++i)
-            if (2 * lane + 64 * i < c.dk) {
-                const float2 vf = load_pair(v + 2 * lane + 64 * i);
-                o[i].x = fmaf(o[i].x, old, p * vf.x);
-                o[i].y = fmaf(o[i].y, old, p * vf.y);
-            }
-        m = top;
-    }
-    for (int i = 0; i < 4; ++i)
-        if (2 * lane + 64 * i < c.dk) {
-            part[warp][2 * lane + 64 * i] = o[i].x;
-            part[warp][2 * lane + 64 * i + 1] = o[i].y;
-        }
-    if (lane == 0) {
-        part[warp][256] = m;
-        part[warp][257] = l;
-    }
-    __syncthreads();
-    float top = -INFINITY, total = 0.0f;
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, part[w][256]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    for (int w = 0; w < 4; ++w) total = fmaf(part[w][257], expf(part[w][256] - base), total);
-    for (int f = threadIdx.x; f < c.dk; f += 128) {
-        float x = 0.0f;
-        for (int w = 0; w < 4; ++w) x = fmaf(part[w][f], expf(part[w][256] - base), x);
-        store_one((TQ*)a.out + (long long)blockIdx.x * c.dk + f, total == 0.0f ? 0.0f : x / total);
-    }
-    if (threadIdx.x == 0) lse_out[blockIdx.x] = total == 0.0f ? -INFINITY : base + logf(total);
-}
-
-// weight[t] += sum over the group of exp(x_t - lse): one CTA per (sequence, KV head), a warp per position
-template <typename TQ, typename TC>
-__global__ void __launch_bounds__(256) paged_weight_kernel(const PagedView c, const SeqView s, const DecodeArgs a, const float* __restrict__ lse, int* flags)
-{
-    const int seq = blockIdx.x / c.heads, hk = blockIdx.x % c.heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n = paged_len(c, s, seq, flags);
-    for (int t = warp; t < n; t += 8) {
-        const long long row = paged_row(s.table[(long long)seq * s.stride + t / c.page], c.n_pages, c.heads, c.page, hk, t % c.page);
-        if (row < 0) continue;
-        const TC* k = (const TC*)c.k + row * c.pitch;
-        float sum = 0.0f;
-        for (int g = 0; g < a.group; ++g) {
-            const int h = hk * a.group + g;
-            const TQ* q = (const TQ*)a.q + (long long)seq * a.q_stride + (long long)h * c.dk;
-            float x = 0.0f;
-            for (int f = 2 * lane; f < c.dk; f += 64) {
-                const float2 kf = load_pair(k + f), qf = load_pair(q + f);
-                x = fmaf(qf.x, kf.x, fmaf(qf.y, kf.y, x));
-            }
-            x = warp_sum(x) * a.scale;
-            const float z = lse[(long long)seq * a.n_head + h];
-            sum += z == -INFINITY ? 0.0f : expf(x - z);
-        }
-        if (lane == 0) atomicAdd(c.w + row, sum);
-    }
-}
-
-// ------------------------------------------------------------------------------------------------ bf16 caches
-// The work is cut evenly whatever the lengths: the positions of every (sequence, KV head) form units of 64, and worker w of G
+// ------------------------------------------------------------------------------------------------ division of the work
+// The work is cut evenly whatever the lengths: the positions of every (sequence, KV head) form units of 64 (32 for wide f32
+// rows), a tile of each unit for each of the CTA's four warps, and worker w of G
 // (one CTA each; G at most U, so that every worker has some) takes the units [U w / G, U (w + 1) / G) of the batch in order.  A worker finishes the
 // (sequence, KV head) items that lie inside its range; of an item that several workers share each leaves a partial softmax
 // (maximum, sum, weighted values) that paged_join_kernel folds in order.  A worker has at most two partial items: slot 0 is
 // one that began in an earlier worker, slot 1 one that begins here and goes on in the next.
-constexpr int UNIT = 64, MAX_CTAS_PER_SM = 4;
+constexpr int MAX_CTAS_PER_SM = 4, MAX_UNIT = 64;
 
 struct DecodeWs {
     int2* desc;      // (G): the split item that begins in worker w and its last worker; item -1: none
@@ -127,7 +39,7 @@ struct DecodeWs {
     float* scores;   // (n_seq, n_head, score_stride): scores in the log2 domain, for the weights; or NULL
     long long score_stride;
     int rows, dkm;   // rows of an item and their pitch in the partial results
-    int slab_groups; // items per (sequence, KV head): groups of more than 16 query heads are cut
+    int slab_groups; // items per (sequence, KV head): larger groups of query heads than a pass serves are cut
 };
 
 // position in the batch's order of units
@@ -135,6 +47,7 @@ struct UnitIter {
     int seq, hs, tile, n, tiles;
 };
 
+template <int UNIT>
 __device__ __forceinline__ void advance(UnitIter& it, const PagedView& c, const SeqView& s, int items_per_seq, int* flags)
 {
     if (++it.tile < it.tiles) return;
@@ -148,6 +61,7 @@ __device__ __forceinline__ void advance(UnitIter& it, const PagedView& c, const 
 }
 
 // Called by all 128 threads: this worker's units and the place of the first one.
+template <int UNIT>
 __device__ __forceinline__ bool find_work(const PagedView& c, const SeqView& s, int items_per_seq, UnitIter& it, long long& u0, long long& u1,
                                           long long& units, int& workers, int* flags)
 {
@@ -235,11 +149,12 @@ __device__ __forceinline__ void cp16_zfill(void* smem, const void* gmem, bool va
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(sa), "l"(gmem), "r"(sz) : "memory");
 }
 
+// ------------------------------------------------------------------------------------------------ bf16 caches
 // What a configuration of the kernel needs.  KS: 16-feature steps of a row (dk padded with zeros in shared memory only);
 // NSLAB: slabs of 8 query heads that share one pass over the cache; PREC: f32 queries and outputs.
 template <int KS, int NSLAB, bool PREC>
 struct MmaCfg {
-    static constexpr int DKM = KS * 16, LD = DKM + 8, TK = 16;
+    static constexpr int DKM = KS * 16, LD = DKM + 8, TK = 16, UNIT = 4 * TK;
     static constexpr bool REGQ = KS * NSLAB * (PREC ? 6 : 4) <= 64;  // query fragments in registers, else in shared memory
     static constexpr int QROWS = REGQ ? 0 : NSLAB * (PREC ? 24 : 16);
     static constexpr int STAGE = 2 * TK * LD;                        // elements of a warp's key and value tile
@@ -268,7 +183,7 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
     UnitIter ct;
     long long u, u1, units;
     int workers;
-    const bool work = find_work(c, s, items_per_seq, ct, u, u1, units, workers, flags);
+    const bool work = find_work<C::UNIT>(c, s, items_per_seq, ct, u, u1, units, workers, flags);
     if (tid == 0) ws.desc[blockIdx.x] = make_int2(-1, -1);
     if (!work) return;
 
@@ -281,7 +196,7 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
     long long iu = u;
     int page_id = -1;
     auto fetch_page = [&]() {
-        const int pos = it.tile * UNIT + warp * TK + (lane & 15);
+        const int pos = it.tile * C::UNIT + warp * TK + (lane & 15);
         if (iu < u1) page_id = pos < it.n ? s.table[(long long)it.seq * s.stride + pos / c.page] : -1;
     };
     fetch_page();
@@ -290,7 +205,7 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
     auto issue = [&](int stage, int age) {
         unsigned mask = 0;
         if (iu < u1) {
-            const int pos = it.tile * UNIT + warp * TK + (lane & 15);
+            const int pos = it.tile * C::UNIT + warp * TK + (lane & 15);
             int row = -1;
             if (pos < it.n) {
                 row = (int)paged_row(page_id, c.n_pages, c.heads, c.page, it.hs / ws.slab_groups, pos % c.page);
@@ -308,7 +223,7 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
                 cp16_zfill(kt + r * LD + ch * 8, kbase + off, ok);
                 cp16_zfill(vt + r * LD + ch * 8, vbase + off, ok);
             }
-            if (++iu < u1) advance(it, c, s, items_per_seq, flags);
+            if (++iu < u1) advance<C::UNIT>(it, c, s, items_per_seq, flags);
             fetch_page();
         }
         exist |= (unsigned long long)mask << (16 * age);
@@ -370,7 +285,7 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
         __syncwarp();
         const __nv_bfloat16* kt = ring + stage * C::STAGE;
         const __nv_bfloat16* vt = kt + TK * LD;
-        const int t0 = ct.tile * UNIT + warp * TK;
+        const int t0 = ct.tile * C::UNIT + warp * TK;
         const unsigned live = (unsigned)exist & 0xffffu;
         exist >>= 16;
         // scores of 16 positions: n-tile j holds positions t0 + 8 j + 2 t4 + {0, 1} of head g
@@ -547,11 +462,290 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
             }
             fresh = true;
         }
-        if (u + 1 < u1) advance(ct, c, s, items_per_seq, flags);
+        if (u + 1 < u1) advance<C::UNIT>(ct, c, s, items_per_seq, flags);
     }
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
 }
 
+// ------------------------------------------------------------------------------------------------ f32 caches
+// The same division of the work with f32 multiply-adds: tensor cores would round the cache.  FL lanes cover a row of V with
+// NFI vectors of four features each; ROWS query heads (at most 8) share a pass.
+template <int FL, int NFI, int ROWS>
+struct FmaCfg {
+    static constexpr int TK = NFI == 2 ? 8 : 16, UNIT = 4 * TK, LPK = 32 / TK, NST = NFI == 2 ? 2 : 3, DKM = FL * 4 * NFI;
+    static constexpr int MB = ROWS * DKM + (2 * ROWS + 3) / 4 * 4;  // a parked partial result: values, then maximum and sum per row
+    // pitch of a row in shared memory: 4 * LPK floats beyond a multiple of 32, so that the keys of a quarter warp, LPK lanes
+    // each, fall on different banks
+    static __host__ __device__ constexpr int ld(int pitch) { return pitch + (4 * LPK + 32 - pitch % 32) % 32; }
+    static __host__ __device__ constexpr size_t smem(int pitch)
+    {
+        return ((size_t)4 * NST * 2 * TK * ld(pitch) + (size_t)ROWS * ld(pitch) + 4 * TK * ROWS + (size_t)2 * MB) * sizeof(float);
+    }
+};
+
+template <int FL, int NFI, int ROWS, typename TQ>
+__global__ void __launch_bounds__(128, 2)
+paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, const DecodeWs ws, int* flags)
+{
+    using C = FmaCfg<FL, NFI, ROWS>;
+    constexpr int TK = C::TK, LPK = C::LPK, NST = C::NST, RPI = 32 / FL;  // RPI: rows that one load instruction covers
+    extern __shared__ __align__(16) float smem_f[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ld = C::ld(c.pitch), stage_len = 2 * TK * ld;
+    float* ring = smem_f + (size_t)warp * NST * stage_len;
+    float* qs = smem_f + (size_t)4 * NST * stage_len;
+    float* ps = qs + (size_t)ROWS * ld + warp * TK * ROWS;  // this warp's probabilities, (position, row)
+    float* mb = qs + (size_t)ROWS * ld + 4 * TK * ROWS;     // two parked partial results
+    pdl_wait();
+    pdl_launch();
+    const int items_per_seq = c.heads * ws.slab_groups;
+    UnitIter ct;
+    long long u, u1, units;
+    int workers;
+    const bool work = find_work<C::UNIT>(c, s, items_per_seq, ct, u, u1, units, workers, flags);
+    if (tid == 0) ws.desc[blockIdx.x] = make_int2(-1, -1);
+    if (!work) return;
+
+    const int chunks = c.pitch / 4, key = lane / LPK, sub = lane % LPK;
+    const float* kbase = (const float*)c.k;
+    const float* vbase = (const float*)c.v;
+    UnitIter it = ct;
+    long long iu = u;
+    int page_id = -1;
+    auto fetch_page = [&]() {
+        const int pos = it.tile * C::UNIT + warp * TK + lane % TK;
+        if (iu < u1) page_id = pos < it.n ? s.table[(long long)it.seq * s.stride + pos / c.page] : -1;
+    };
+    fetch_page();
+    unsigned long long exist = 0;  // as in the bf16 kernel
+    auto issue = [&](int stage, int age) {
+        unsigned mask = 0;
+        if (iu < u1) {
+            const int pos = it.tile * C::UNIT + warp * TK + lane % TK;
+            int row = -1;
+            if (pos < it.n) {
+                row = (int)paged_row(page_id, c.n_pages, c.heads, c.page, it.hs / ws.slab_groups, pos % c.page);
+                if (row < 0) paged_flag(flags, PAGED_BAD_PAGE);
+            }
+            mask = __ballot_sync(0xffffffffu, row >= 0) & ((1u << TK) - 1u);
+            float* kt = ring + stage * stage_len;
+            float* vt = kt + TK * ld;
+#pragma unroll
+            for (int i = 0; i < TK / RPI; ++i) {
+                const int r = i * RPI + lane / FL;
+                const int src = __shfl_sync(0xffffffffu, row, r);
+#pragma unroll
+                for (int j = 0; j < NFI; ++j) {
+                    const int ch = lane % FL + FL * j;
+                    if (ch < chunks) {
+                        const size_t off = src >= 0 ? (size_t)src * c.pitch + ch * 4 : 0;
+                        cp16_zfill(kt + r * ld + ch * 4, kbase + off, src >= 0);
+                        cp16_zfill(vt + r * ld + ch * 4, vbase + off, src >= 0);
+                    }
+                }
+            }
+            if (++iu < u1) advance<C::UNIT>(it, c, s, items_per_seq, flags);
+            fetch_page();
+        }
+        exist |= (unsigned long long)mask << (16 * age);
+        asm volatile("cp.async.commit_group;\n" ::);
+    };
+#pragma unroll
+    for (int i = 0; i < NST; ++i) issue(i, i);
+
+    const float scale2 = a.scale * 1.44269504088896341f;
+    float4 o[ROWS][NFI];
+    float m[ROWS], l[ROWS];  // l: this lane's share
+    bool fresh = true, starts_here = false;
+    int stage = 0, slot = 0;
+    for (; u < u1; ++u) {
+        const int hk = ct.hs / ws.slab_groups, row0 = (ct.hs % ws.slab_groups) * ROWS;
+        if (fresh) {
+            fresh = false;
+            starts_here = ct.tile == 0;
+            slot = starts_here ? 1 : 0;
+            const TQ* q = (const TQ*)a.q + (long long)ct.seq * a.q_stride + (long long)(hk * a.group + row0) * c.dk;
+            __syncthreads();
+            for (int i = tid; i < ROWS * c.pitch; i += 128) {
+                const int r = i / c.pitch, f = i % c.pitch;
+                qs[r * ld + f] = row0 + r < a.group && f < c.dk ? load_one(q + r * c.dk + f) : 0.0f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                m[r] = -INFINITY;
+                l[r] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < NFI; ++j) o[r][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        }
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 1) : "memory");
+        __syncwarp();
+        const float* kt = ring + stage * stage_len;
+        const float* vt = kt + TK * ld;
+        const int t0 = ct.tile * C::UNIT + warp * TK;
+        const unsigned live = (unsigned)exist & 0xffffu;
+        exist >>= 16;
+        // scores: LPK lanes per position, every LPK-th vector of the row each
+        float x[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) x[r] = 0.0f;
+        for (int ch = sub; ch < chunks; ch += LPK) {
+            const float4 kf = *reinterpret_cast<const float4*>(kt + key * ld + ch * 4);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const float4 qf = *reinterpret_cast<const float4*>(qs + r * ld + ch * 4);
+                x[r] = fmaf(qf.x, kf.x, fmaf(qf.y, kf.y, fmaf(qf.z, kf.z, fmaf(qf.w, kf.w, x[r]))));
+            }
+        }
+        const bool on = (live >> key) & 1u;
+        float corr[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+            for (int d = 1; d < LPK; d <<= 1) x[r] += __shfl_xor_sync(0xffffffffu, x[r], d);
+            x[r] = on ? __fmul_rn(x[r], scale2) : -INFINITY;
+            if (ws.scores && sub == 0 && row0 + r < a.group)
+                ws.scores[((long long)ct.seq * a.n_head + hk * a.group + row0 + r) * ws.score_stride + t0 + key] = x[r];
+            float top = x[r];
+#pragma unroll
+            for (int d = LPK; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            top = fmaxf(top, m[r]);
+            const float base = top == -INFINITY ? 0.0f : top;
+            corr[r] = exp2f(m[r] - base);
+            m[r] = top;
+            x[r] = exp2f(x[r] - base);
+            l[r] = fmaf(l[r], corr[r], x[r]);  // the LPK lanes of a position hold the same share: divided out at the end
+            if (sub == 0) ps[key * ROWS + r] = x[r];
+        }
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int j = 0; j < NFI; ++j) {
+                o[r][j].x *= corr[r];
+                o[r][j].y *= corr[r];
+                o[r][j].z *= corr[r];
+                o[r][j].w *= corr[r];
+            }
+#pragma unroll
+        for (int i = 0; i < TK / RPI; ++i) {
+            const int t = i * RPI + lane / FL;
+#pragma unroll
+            for (int j = 0; j < NFI; ++j) {
+                const int ch = lane % FL + FL * j;
+                if (ch < chunks) {
+                    const float4 vf = *reinterpret_cast<const float4*>(vt + t * ld + ch * 4);
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r) {
+                        const float p = ps[t * ROWS + r];
+                        o[r][j].x = fmaf(p, vf.x, o[r][j].x);
+                        o[r][j].y = fmaf(p, vf.y, o[r][j].y);
+                        o[r][j].z = fmaf(p, vf.z, o[r][j].z);
+                        o[r][j].w = fmaf(p, vf.w, o[r][j].w);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        issue(stage, NST - 1);
+        stage = stage + 1 == NST ? 0 : stage + 1;
+
+        const bool ends = ct.tile + 1 == ct.tiles;
+        if (ends || u + 1 == u1) {  // fold the lanes' and the warps' results; warp 0 writes
+            const bool whole = starts_here && ends;
+            if (tid == 0 && starts_here && !ends)
+                ws.desc[blockIdx.x] = make_int2(ct.seq * items_per_seq + ct.hs, worker_of(u + (ct.tiles - 1 - ct.tile), units, workers));
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                l[r] = warp_sum(l[r]) * (1.0f / LPK);
+#pragma unroll
+                for (int j = 0; j < NFI; ++j)
+#pragma unroll
+                    for (int d = FL; d < 32; d <<= 1) {
+                        o[r][j].x += __shfl_xor_sync(0xffffffffu, o[r][j].x, d);
+                        o[r][j].y += __shfl_xor_sync(0xffffffffu, o[r][j].y, d);
+                        o[r][j].z += __shfl_xor_sync(0xffffffffu, o[r][j].z, d);
+                        o[r][j].w += __shfl_xor_sync(0xffffffffu, o[r][j].w, d);
+                    }
+            }
+            auto park = [&](float* buf) {
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    if (lane < FL)
+#pragma unroll
+                        for (int j = 0; j < NFI; ++j) *reinterpret_cast<float4*>(buf + r * C::DKM + (lane + FL * j) * 4) = o[r][j];
+                    if (lane == 0) {
+                        buf[ROWS * C::DKM + 2 * r] = m[r];
+                        buf[ROWS * C::DKM + 2 * r + 1] = l[r];
+                    }
+                }
+            };
+            auto fold = [&](const float* buf) {
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    const float mo = buf[ROWS * C::DKM + 2 * r], lo = buf[ROWS * C::DKM + 2 * r + 1];
+                    const float top = fmaxf(m[r], mo), base = top == -INFINITY ? 0.0f : top;
+                    const float ca = exp2f(m[r] - base), cb = exp2f(mo - base);
+                    m[r] = top;
+                    l[r] = fmaf(l[r], ca, lo * cb);
+#pragma unroll
+                    for (int j = 0; j < NFI; ++j) {
+                        const float4 y = *reinterpret_cast<const float4*>(buf + r * C::DKM + (lane % FL + FL * j) * 4);
+                        o[r][j].x = fmaf(o[r][j].x, ca, y.x * cb);
+                        o[r][j].y = fmaf(o[r][j].y, ca, y.y * cb);
+                        o[r][j].z = fmaf(o[r][j].z, ca, y.z * cb);
+                        o[r][j].w = fmaf(o[r][j].w, ca, y.w * cb);
+                    }
+                }
+            };
+            __syncthreads();
+            if (warp >= 2) park(mb + (warp - 2) * C::MB);
+            __syncthreads();
+            if (warp < 2) fold(mb + warp * C::MB);
+            __syncthreads();
+            if (warp == 1) park(mb);
+            __syncthreads();
+            if (warp == 0) {
+                fold(mb);
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    if (row0 + r >= a.group) continue;
+                    const long long hq = (long long)ct.seq * a.n_head + hk * a.group + row0 + r;
+                    const long long pr = ((long long)blockIdx.x * 2 + slot) * ws.rows + r;
+                    const float inv = l[r] == 0.0f ? 0.0f : __fdiv_rn(1.0f, l[r]);
+#pragma unroll
+                    for (int j = 0; j < NFI; ++j) {
+                        const int f = (lane + FL * j) * 4;
+                        if (lane >= FL) continue;
+                        if (!whole) {
+                            *reinterpret_cast<float4*>(ws.o + pr * ws.dkm + f) = o[r][j];
+                        } else {
+                            const float v[4] = {o[r][j].x, o[r][j].y, o[r][j].z, o[r][j].w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (f + i < c.dk) store_one((TQ*)a.out + hq * c.dk + f + i, v[i] * inv);
+                        }
+                    }
+                    if (lane == 0) {
+                        if (!whole) {
+                            ws.ml[pr * 2] = m[r];
+                            ws.ml[pr * 2 + 1] = l[r];
+                        } else {
+                            const float z = l[r] == 0.0f ? -INFINITY : m[r] + log2f(l[r]);
+                            if (a.lse) a.lse[hq] = z * 0.693147180559945309f;
+                            if (ws.lse2) ws.lse2[hq] = z;
+                        }
+                    }
+                }
+            }
+            fresh = true;
+        }
+        if (u + 1 < u1) advance<C::UNIT>(ct, c, s, items_per_seq, flags);
+    }
+    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+}
+
+// ------------------------------------------------------------------------------------------------ joining
 // One CTA per (worker whose last item goes on, row of the item): folds the partial results of workers w .. last.  Also
 // answers for the sequences without any position.
 template <typename TQ>
@@ -656,13 +850,18 @@ struct WsPlan {
     int rows, dkm, slab_groups;
     long long score_stride;
 };
-static WsPlan plan_ws(int sm_count, const PagedView& c, const SeqView& s, size_t n_head, bool accumulate)
+static WsPlan plan_ws(int sm_count, bool f32_cache, const PagedView& c, const SeqView& s, size_t n_head, bool accumulate)
 {
     const int group = (int)(n_head / c.heads);
     WsPlan p{};
-    p.rows = group > 8 ? 16 : 8;
-    p.slab_groups = (group + 15) / 16;
-    p.dkm = c.dk <= 64 ? 64 : c.dk <= 112 ? 112 : c.dk <= 128 ? 128 : c.dk <= 192 ? 192 : 256;
+    if (f32_cache) {
+        p.rows = group == 1 ? 1 : group == 2 ? 2 : group <= 4 ? 4 : 8;
+        p.dkm = c.dk <= 64 ? 64 : c.dk <= 128 ? 128 : 256;
+    } else {
+        p.rows = group > 8 ? 16 : 8;
+        p.dkm = c.dk <= 64 ? 64 : c.dk <= 112 ? 112 : c.dk <= 128 ? 128 : c.dk <= 192 ? 192 : 256;
+    }
+    p.slab_groups = (group + p.rows - 1) / p.rows;
     const size_t g = (size_t)sm_count * MAX_CTAS_PER_SM;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     p.desc = 0;
@@ -670,7 +869,7 @@ static WsPlan plan_ws(int sm_count, const PagedView& c, const SeqView& s, size_t
     p.o = p.ml + up(g * 2 * p.rows * 2 * sizeof(float));
     p.lse2 = p.o + up(g * 2 * p.rows * p.dkm * sizeof(float));
     p.scores = p.lse2 + (accumulate ? up(s.n_seq * n_head * sizeof(float)) : 0);
-    p.score_stride = (paged_capacity(c, s) + UNIT - 1) / UNIT * UNIT;
+    p.score_stride = (paged_capacity(c, s) + MAX_UNIT - 1) / MAX_UNIT * MAX_UNIT;
     p.total = p.scores + (accumulate ? s.n_seq * n_head * (size_t)p.score_stride * sizeof(float) : 0);
     return p;
 }
@@ -683,64 +882,79 @@ struct PdlOn {
     ~PdlOn() { e->pdl = prev; }
 };
 
-template <int KS, int NSLAB, typename TQ>
-static nnb_status launch_mma(nnb_engine* e, const PagedView& c, const SeqView& s, const DecodeArgs& a, const DecodeWs& ws, int* workers)
+template <typename... K>
+static nnb_status launch_workers(nnb_engine* e, void (*kern)(K...), size_t smem, int (&per_sm)[64], const PagedView& c, const SeqView& s, const DecodeArgs& a,
+                                 const DecodeWs& ws, int* workers)
 {
-    using C = MmaCfg<KS, NSLAB, sizeof(TQ) == 4>;
-    auto kern = paged_decode_mma_kernel<KS, NSLAB, TQ>;
-    static int per_sm[64] = {};  // resident CTAs per SM, by device
-    int& n = per_sm[e->device & 63];
+    int& n = per_sm[e->device & 63];  // resident CTAs per SM, by device
     if (n == 0) {
-        NNB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
-        NNB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, 128, C::SMEM));
+        NNB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        NNB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, 128, smem));
         n = n < 1 ? 1 : n > MAX_CTAS_PER_SM ? MAX_CTAS_PER_SM : n;
     }
     *workers = e->sm_count * n;
-    NNB_CUDA(launch_ex(e, kern, dim3((unsigned)*workers), dim3(128), C::SMEM, c, s, a, ws, e->dev_flags));
+    NNB_CUDA(launch_ex(e, kern, dim3((unsigned)*workers), dim3(128), smem, c, s, a, ws, e->dev_flags));
     e->launches++;
     return NNB_OK;
 }
-template <typename TQ>
-static nnb_status launch_decode_b16(nnb_engine* e, const PagedView& c, const SeqView& s, const DecodeArgs& a, bool accumulate, char* base)
+template <int KS, typename TQ>
+static nnb_status launch_mma(nnb_engine* e, const PagedView& c, const SeqView& s, const DecodeArgs& a, const DecodeWs& ws, int* workers)
 {
-    const WsPlan p = plan_ws(e->sm_count, c, s, (size_t)a.n_head, accumulate);
+    static int one[64] = {}, two[64] = {};
+    if (ws.rows == 16)
+        return launch_workers(e, paged_decode_mma_kernel<KS, 2, TQ>, MmaCfg<KS, 2, sizeof(TQ) == 4>::SMEM, two, c, s, a, ws, workers);
+    return launch_workers(e, paged_decode_mma_kernel<KS, 1, TQ>, MmaCfg<KS, 1, sizeof(TQ) == 4>::SMEM, one, c, s, a, ws, workers);
+}
+template <int FL, int NFI, int ROWS, typename TQ>
+static nnb_status launch_fma_rows(nnb_engine* e, const PagedView& c, const SeqView& s, const DecodeArgs& a, const DecodeWs& ws, int* workers)
+{
+    static int per_sm[64] = {};
+    // one size for all rows that these lanes cover, so that residency is a property of the kernel
+    return launch_workers(e, paged_decode_fma_kernel<FL, NFI, ROWS, TQ>, FmaCfg<FL, NFI, ROWS>::smem(FL * 4 * NFI), per_sm, c, s, a, ws, workers);
+}
+template <int FL, int NFI, typename TQ>
+static nnb_status launch_fma(nnb_engine* e, const PagedView& c, const SeqView& s, const DecodeArgs& a, const DecodeWs& ws, int* workers)
+{
+    switch (ws.rows) {
+        case 1: return launch_fma_rows<FL, NFI, 1, TQ>(e, c, s, a, ws, workers);
+        case 2: return launch_fma_rows<FL, NFI, 2, TQ>(e, c, s, a, ws, workers);
+        case 4: return launch_fma_rows<FL, NFI, 4, TQ>(e, c, s, a, ws, workers);
+        default: return launch_fma_rows<FL, NFI, 8, TQ>(e, c, s, a, ws, workers);
+    }
+}
+template <typename TQ>
+static nnb_status launch_decode(nnb_engine* e, bool f32_cache, const PagedView& c, const SeqView& s, const DecodeArgs& a, bool accumulate, char* base)
+{
+    const WsPlan p = plan_ws(e->sm_count, f32_cache, c, s, (size_t)a.n_head, accumulate);
     const DecodeWs ws{(int2*)(base + p.desc), (float*)(base + p.ml), (float*)(base + p.o), accumulate ? (float*)(base + p.lse2) : nullptr,
                       accumulate ? (float*)(base + p.scores) : nullptr, p.score_stride, p.rows, p.dkm, p.slab_groups};
     PdlOn pdl(e);
     int workers = 0;
-    const bool two = p.rows == 16;
-#define NNB_MMA(KS) NNB_TRY((two ? launch_mma<KS, 2, TQ>(e, c, s, a, ws, &workers) : launch_mma<KS, 1, TQ>(e, c, s, a, ws, &workers)))
-    switch (p.dkm) {
-        case 64: NNB_MMA(4); break;
-        case 112: NNB_MMA(7); break;
-        case 128: NNB_MMA(8); break;
-        case 192: NNB_MMA(12); break;
-        default: NNB_MMA(16); break;
+    if (f32_cache) {
+        if (p.dkm == 64)
+            NNB_TRY((launch_fma<16, 1, TQ>(e, c, s, a, ws, &workers)));
+        else if (p.dkm == 128)
+            NNB_TRY((launch_fma<32, 1, TQ>(e, c, s, a, ws, &workers)));
+        else
+            NNB_TRY((launch_fma<32, 2, TQ>(e, c, s, a, ws, &workers)));
+    } else {
+        switch (p.dkm) {
+            case 64: NNB_TRY((launch_mma<4, TQ>(e, c, s, a, ws, &workers))); break;
+            case 112: NNB_TRY((launch_mma<7, TQ>(e, c, s, a, ws, &workers))); break;
+            case 128: NNB_TRY((launch_mma<8, TQ>(e, c, s, a, ws, &workers))); break;
+            case 192: NNB_TRY((launch_mma<12, TQ>(e, c, s, a, ws, &workers))); break;
+            default: NNB_TRY((launch_mma<16, TQ>(e, c, s, a, ws, &workers))); break;
+        }
     }
-#undef NNB_MMA
     const size_t smem = (size_t)(workers > 512 ? workers : 512) * sizeof(float);
-    NNB_CUDA(launch_ex(e, paged_join_kernel<TQ>, dim3((unsigned)workers, (unsigned)(a.group < p.rows ? a.group : p.rows)), dim3(128), smem, c, s, a, ws, e->dev_flags));
+    NNB_CUDA(launch_ex(e, paged_join_kernel<TQ>, dim3((unsigned)workers, (unsigned)(a.group < p.rows ? a.group : p.rows)), dim3(128), smem, c, s, a, ws,
+                       e->dev_flags));
     e->launches++;
     if (accumulate) {
         const unsigned items = (unsigned)(s.n_seq * c.heads);
         const size_t want = ceil_div((size_t)e->sm_count * 8, items), most = ceil_div((size_t)paged_capacity(c, s), 256);
         NNB_CUDA(launch_ex(e, paged_add_weights_kernel, dim3(items, (unsigned)(want < most ? want : most)), dim3(256), 0, c, s, a, ws, e->dev_flags));
         e->launches++;
-    }
-    return NNB_OK;
-}
-
-template <typename TQ, typename TC>
-static nnb_status launch_decode(nnb_engine* e, const PagedView& c, const SeqView& s, const DecodeArgs& a, bool accumulate, float* ws)
-{
-    float* lse = a.lse ? a.lse : ws;
-    paged_decode_kernel<TQ, TC><<<(unsigned)(s.n_seq * a.n_head), 128, 0, e->stream>>>(c, s, a, lse, e->dev_flags);
-    e->launches++;
-    NNB_CHECK_LAUNCH("paged_decode_kernel");
-    if (accumulate) {
-        paged_weight_kernel<TQ, TC><<<(unsigned)(s.n_seq * c.heads), 256, 0, e->stream>>>(c, s, a, lse, e->dev_flags);
-        e->launches++;
-        NNB_CHECK_LAUNCH("paged_weight_kernel");
     }
     return NNB_OK;
 }
@@ -758,8 +972,7 @@ size_t nnb_paged_attention_workspace(nnb_engine* e, const nnb_paged_cache* c, co
     if (!e || paged_check_cache("paged_attention_decode", c, &cv) != NNB_OK || paged_check_seqs("paged_attention_decode", c, s, &sv) != NNB_OK ||
         n_head == 0 || n_head % cv.heads != 0)
         return 0;
-    const size_t simple = (size_t)sv.n_seq * n_head * sizeof(float);
-    return c->dtype == NNB_F32 ? simple + 16 : plan_ws(e->sm_count, cv, sv, n_head, accumulate != 0).total;
+    return plan_ws(e->sm_count, c->dtype == NNB_F32, cv, sv, n_head, accumulate != 0).total;
 }
 
 nnb_status nnb_paged_attention_decode(nnb_engine* e, const nnb_paged_cache* c, const nnb_paged_seqs* s, const void* d_q, int dtype,
@@ -786,13 +999,8 @@ nnb_status nnb_paged_attention_decode(nnb_engine* e, const nnb_paged_cache* c, c
                 "%s: the workspace is too small", who);
     DeviceScope dev(e->device);
     const DecodeArgs a{d_q, (long long)q_stride, (int)n_head, (int)(n_head / cv.heads), scale != 0.0f ? scale : 1.0f / sqrtf((float)cv.dk), d_out, d_lse};
-    const bool acc = accumulate != 0;
-    if (dtype == NNB_F32) {
-        if (c->dtype == NNB_F32) return launch_decode<float, float>(e, cv, sv, a, acc, (float*)d_ws);
-        return launch_decode_b16<float>(e, cv, sv, a, acc, (char*)d_ws);
-    }
-    if (c->dtype == NNB_F32) return launch_decode<__nv_bfloat16, float>(e, cv, sv, a, acc, (float*)d_ws);
-    return launch_decode_b16<__nv_bfloat16>(e, cv, sv, a, acc, (char*)d_ws);
+    if (dtype == NNB_F32) return launch_decode<float>(e, c->dtype == NNB_F32, cv, sv, a, accumulate != 0, (char*)d_ws);
+    return launch_decode<__nv_bfloat16>(e, c->dtype == NNB_F32, cv, sv, a, accumulate != 0, (char*)d_ws);
 }
 
 }  // extern "C"

@@ -52,7 +52,8 @@ class PagedCache:
         _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.dtype in _DTYPES,
               "keys and values are (n_pages, n_head_kv, page_size, pitch) tensors of one shape and type, f32 or bf16")
         dk = k.shape[3] if dk is None else int(dk)
-        _need(k.shape[3] == (dk + 7) // 8 * 8, f"a head size of {dk} needs rows of {(dk + 7) // 8 * 8} features, not {k.shape[3]}")
+        if k.shape[3] != (dk + 7) // 8 * 8:
+            raise NnbError(f"a head size of {dk} needs rows of {(dk + 7) // 8 * 8} features, not {k.shape[3]}")
         _need(weight is None or (weight.shape == k.shape[:3] and weight.dtype == torch.float32), "weights are (n_pages, n_head_kv, page_size) f32")
         for t in (k, v) if weight is None else (k, v, weight):
             _need(t.is_cuda and t.is_contiguous() and t.device == k.device, "the cache consists of contiguous CUDA tensors of one device")
@@ -74,57 +75,59 @@ class PagedCache:
         return int(lib().nnb_paged_row(C.byref(self._c), ids, len(table_row), head, pos))
 
 
-class _Ordered:
-    """Orders a call with torch's current stream where the engine launches on another one."""
-
-    __slots__ = ("cur", "own")
-
-    def __init__(self, eng):
-        self.cur = torch.cuda.current_stream(eng.device)
-        ptr = eng._lib.nnb_engine_stream(eng._h) or 0
-        self.own = None if ptr == self.cur.cuda_stream else torch.cuda.ExternalStream(ptr, device=eng.device)
-
-    def __enter__(self):
-        if self.own is not None:
-            self.own.wait_stream(self.cur)
-
-    def __exit__(self, *exc):
-        if self.own is not None:
-            self.cur.wait_stream(self.own)
+def _call(eng, fn, *args):
+    """fn(engine, *args), ordered with torch's current stream where the engine launches on another one."""
+    ptr = eng._lib.nnb_engine_stream(eng._h) or 0
+    if ptr == torch._C._cuda_getCurrentRawStream(eng.device.index):
+        check(fn(eng._h, *args))
+        return
+    cur, own = torch.cuda.current_stream(eng.device), torch.cuda.ExternalStream(ptr, device=eng.device)
+    own.wait_stream(cur)
+    try:
+        check(fn(eng._h, *args))
+    finally:
+        cur.wait_stream(own)
 
 
+# The checks below run on every call: messages are only put together when one fails.
 def _on(eng, name, t, dtype, shape=None):
-    _need(t.device == eng.device, f"{name} is on {t.device}, the engine on {eng.device}")
-    _need(t.dtype == dtype, f"{name} is {t.dtype}, not {dtype}")
-    _need(shape is None or tuple(t.shape) == shape, f"{name} has shape {tuple(t.shape)}, not {shape}")
+    if t.device != eng.device:
+        raise NnbError(f"{name} is on {t.device}, the engine on {eng.device}")
+    if t.dtype != dtype:
+        raise NnbError(f"{name} is {t.dtype}, not {dtype}")
+    if shape is not None and t.shape != shape:
+        raise NnbError(f"{name} has shape {tuple(t.shape)}, not {shape}")
     return t
 
 
 def _flat(eng, name, t, dtype, shape):
-    _need(_on(eng, name, t, dtype, shape).is_contiguous(), f"{name} is not contiguous")
+    if not _on(eng, name, t, dtype, shape).is_contiguous():
+        raise NnbError(f"{name} is not contiguous")
     return t.data_ptr()
 
 
 def _rows(eng, name, t, heads=None, dk=None):
     """(rows, heads, dk) with contiguous rows, any distance apart; returns the distance in elements."""
-    _need(t.device == eng.device, f"{name} is on {t.device}, the engine on {eng.device}")
-    _need(t.dim() == 3 and t.dtype in _DTYPES, f"{name} is a (rows, heads, dk) tensor, f32 or bf16")
-    _need((heads is None or t.shape[1] == heads) and (dk is None or t.shape[2] == dk), f"{name} has shape {tuple(t.shape)}")
-    _need(t.numel() == 0 or (t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == t.shape[2]) and t.stride(0) >= 0),
-          f"the rows of {name} are not contiguous")
-    return t.stride(0)
+    if t.device != eng.device:
+        raise NnbError(f"{name} is on {t.device}, the engine on {eng.device}")
+    shape = t.shape
+    if len(shape) != 3 or t.dtype not in _DTYPES:
+        raise NnbError(f"{name} is a (rows, heads, dk) tensor, f32 or bf16")
+    if (heads is not None and shape[1] != heads) or (dk is not None and shape[2] != dk):
+        raise NnbError(f"{name} has shape {tuple(shape)}")
+    row, head, one = t.stride()
+    if (one != 1 or (shape[1] != 1 and head != shape[2]) or row < 0) and t.numel():
+        raise NnbError(f"the rows of {name} are not contiguous")
+    return row
 
 
 def _seqs(eng, cache, table, lengths):
-    _need(cache.k.device == eng.device, f"the cache is on {cache.k.device}, the engine on {eng.device}")
-    _need(_on(eng, "table", table, torch.int32).dim() == 2 and (table.numel() == 0 or table.stride(1) == 1), "table is (n_seq, max_pages) with contiguous rows")
-    n = table.shape[0]
-    stride = table.stride(0) if n > 1 else table.shape[1]
-    return _Seqs(table.data_ptr(), _flat(eng, "lengths", lengths, torch.int32, (n,)), n, table.shape[1], stride)
-
-
-def _workspace(eng, size):
-    return torch.empty(size, device=eng.device, dtype=torch.uint8)
+    if cache.k.device != eng.device:
+        raise NnbError(f"the cache is on {cache.k.device}, the engine on {eng.device}")
+    if _on(eng, "table", table, torch.int32).dim() != 2 or (table.stride(1) != 1 and table.numel()):
+        raise NnbError("table is (n_seq, max_pages) with contiguous rows")
+    n, cols = table.shape
+    return _Seqs(table.data_ptr(), _flat(eng, "lengths", lengths, torch.int32, (n,)), n, cols, table.stride(0) if n > 1 else cols)
 
 
 def paged_append(self, cache, table, lengths, k, v, q=None, row_start=None, rope=None, positions=None, q_out=None, lengths_out=None):
@@ -134,15 +137,20 @@ def paged_append(self, cache, table, lengths, k, v, q=None, row_start=None, rope
     s = _seqs(self, cache, table, lengths)
     rows, n = k.shape[0], s.n_seq
     ks, vs = _rows(self, "k", k, cache.n_head_kv, cache.dk), _rows(self, "v", v, cache.n_head_kv, cache.dk)
-    _need(v.shape[0] == rows and v.dtype == k.dtype, "k and v differ in rows or type")
+    if v.shape[0] != rows or v.dtype != k.dtype:
+        raise NnbError("k and v differ in rows or type")
     t = _Tokens(None, k.data_ptr(), v.data_ptr(), None, 0, ks, vs, 0, _DTYPES[k.dtype], 0, rows, None, None, None, None, 0)
     if q is not None:
         t.q_stride = _rows(self, "q", q, None, cache.dk)
-        _need(q.shape[0] == rows and q.dtype == k.dtype, "q and k differ in rows or type")
+        if q.shape[0] != rows or q.dtype != k.dtype:
+            raise NnbError("q and k differ in rows or type")
         if q_out is None:
-            q_out = torch.empty(q.shape, device=self.device, dtype=q.dtype)
-        _need(q_out.shape == q.shape and q_out.dtype == q.dtype, "q_out and q differ in shape or type")
-        t.q_out_stride, t.n_head, t.d_q, t.d_q_out = _rows(self, "q_out", q_out), q.shape[1], q.data_ptr(), q_out.data_ptr()
+            q_out, t.q_out_stride = q.new_empty(q.shape), q.shape[1] * q.shape[2]
+        else:
+            t.q_out_stride = _rows(self, "q_out", q_out)
+            if q_out.shape != q.shape or q_out.dtype != q.dtype:
+                raise NnbError("q_out and q differ in shape or type")
+        t.n_head, t.d_q, t.d_q_out = q.shape[1], q.data_ptr(), q_out.data_ptr()
     else:
         q_out = None
     if row_start is not None:
@@ -156,8 +164,7 @@ def paged_append(self, cache, table, lengths, k, v, q=None, row_start=None, rope
     if lengths_out is None:
         lengths_out = torch.empty_like(lengths)
     out = _flat(self, "lengths_out", lengths_out, torch.int32, (n,))
-    with _Ordered(self):
-        check(self._lib.nnb_paged_append(self._h, C.byref(cache._c), C.byref(s), C.byref(t), out))
+    _call(self, self._lib.nnb_paged_append, C.byref(cache._c), C.byref(s), C.byref(t), out)
     return q_out, lengths_out
 
 
@@ -167,17 +174,21 @@ def paged_attention_decode(self, cache, table, lengths, q, scale=0.0, accumulate
     s = _seqs(self, cache, table, lengths)
     stride = _rows(self, "q", q, None, cache.dk)
     n, heads = s.n_seq, q.shape[1]
-    _need(q.shape[0] == n, f"{q.shape[0]} queries for {n} sequences")
+    if q.shape[0] != n:
+        raise NnbError(f"{q.shape[0]} queries for {n} sequences")
     if out is None:
-        out = torch.empty(q.shape, device=self.device, dtype=q.dtype)
+        out = q.new_empty(q.shape)
+    else:
+        _flat(self, "out", out, q.dtype, q.shape)
     if lse is None:
-        lse = torch.empty((n, heads), device=self.device, dtype=torch.float32)
-    d_out, d_lse = _flat(self, "out", out, q.dtype, tuple(q.shape)), _flat(self, "lse", lse, torch.float32, (n, heads))
-    size = self._lib.nnb_paged_attention_workspace(self._h, C.byref(cache._c), C.byref(s), heads, int(accumulate))
-    ws = _workspace(self, size)
-    with _Ordered(self):
-        check(self._lib.nnb_paged_attention_decode(self._h, C.byref(cache._c), C.byref(s), q.data_ptr(), _DTYPES[q.dtype], stride, heads, scale, d_out,
-                                                   d_lse, int(accumulate), ws.data_ptr(), size))
+        lse = q.new_empty((n, heads), dtype=torch.float32)
+    else:
+        _flat(self, "lse", lse, torch.float32, (n, heads))
+    accumulate, d_out, d_lse = int(accumulate), out.data_ptr(), lse.data_ptr()
+    size = self._lib.nnb_paged_attention_workspace(self._h, C.byref(cache._c), C.byref(s), heads, accumulate)
+    ws = q.new_empty(size, dtype=torch.uint8)
+    _call(self, self._lib.nnb_paged_attention_decode, C.byref(cache._c), C.byref(s), q.data_ptr(), _DTYPES[q.dtype], stride, heads, scale, d_out, d_lse,
+          accumulate, ws.data_ptr(), size)
     return out, lse
 
 
@@ -191,10 +202,9 @@ def paged_evict(self, cache, table, lengths, dst, dst_table, budget, sinks=0, re
     n_out = _flat(self, "lengths_out", lengths_out, torch.int32, (s.n_seq,))
     _need(budget >= 0 and sinks >= 0 and recent >= 0, "budget, sinks and recent are not negative")
     size = self._lib.nnb_paged_evict_workspace(self._h, C.byref(cache._c), C.byref(s), budget)
-    ws = _workspace(self, size)
-    with _Ordered(self):
-        check(self._lib.nnb_paged_evict(self._h, C.byref(cache._c), C.byref(s), budget, sinks, recent, C.byref(dst._c), d.d_table, d.max_pages,
-                                        d.table_stride, n_out, ws.data_ptr(), size))
+    ws = lengths.new_empty(size, dtype=torch.uint8)
+    _call(self, self._lib.nnb_paged_evict, C.byref(cache._c), C.byref(s), budget, sinks, recent, C.byref(dst._c), d.d_table, d.max_pages, d.table_stride,
+          n_out, ws.data_ptr(), size)
     return lengths_out
 
 
@@ -206,8 +216,9 @@ def adjust_logits(self, logits, history=None, history_len=None, prompt_len=None,
     _need(logits.dim() == 2 and logits.dtype in _DTYPES and logits.device == self.device, "logits is an (n_seq, vocab) tensor on the engine's device, f32 or bf16")
     n, vocab = logits.shape
     if out is None:
-        out = torch.empty((n, vocab), device=self.device, dtype=logits.dtype)
-    _on(self, "out", out, logits.dtype, (n, vocab))
+        out = logits.new_empty((n, vocab))
+    else:
+        _on(self, "out", out, logits.dtype, (n, vocab))
     _need(n == 0 or (logits.stride(1) == 1 and out.stride(1) == 1), "rows of the logits are not contiguous")
     c = _Logits()
     c.repeat_window = repeat_window
@@ -230,12 +241,11 @@ def adjust_logits(self, logits, history=None, history_len=None, prompt_len=None,
     for name, t, dtype, width in (("bias", bias, torch.float32, vocab), ("allowed", allowed, torch.int32, (vocab + 31) // 32)):
         if t is not None:
             _on(self, name, t, dtype)
-            _need(tuple(t.shape) in ((width,), (n, width)) and t.stride(-1) == 1, f"{name} is ({width}) or ({n}, {width}) with contiguous rows")
+            if tuple(t.shape) not in ((width,), (n, width)) or t.stride(-1) != 1:
+                raise NnbError(f"{name} is ({width}) or ({n}, {width}) with contiguous rows")
             setattr(c, "d_" + name, t.data_ptr())
             setattr(c, name + "_stride", t.stride(0) if t.dim() == 2 else 0)
-    with _Ordered(self):
-        check(self._lib.nnb_adjust_logits(self._h, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, logits.stride(0), C.byref(c), out.data_ptr(),
-                                          out.stride(0)))
+    _call(self, self._lib.nnb_adjust_logits, logits.data_ptr(), _DTYPES[logits.dtype], n, vocab, logits.stride(0), C.byref(c), out.data_ptr(), out.stride(0))
     return out
 
 
