@@ -23,54 +23,63 @@ __device__ __forceinline__ void store_one(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_one(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
 // ------------------------------------------------------------------------------------------------ division of the work
-// The work is cut evenly whatever the lengths: the positions of every (sequence, KV head) form units of 64 (32 for wide f32
-// rows), a tile of each unit for each of the CTA's four warps, and worker w of G
-// (one CTA each; G at most U, so that every worker has some) takes the units [U w / G, U (w + 1) / G) of the batch in order.  A worker finishes the
-// (sequence, KV head) items that lie inside its range; of an item that several workers share each leaves a partial softmax
-// (maximum, sum, weighted values) that paged_join_kernel folds in order.  A worker has at most two partial items: slot 0 is
-// one that began in an earlier worker, slot 1 one that begins here and goes on in the next.
-constexpr int MAX_CTAS_PER_SM = 4, MAX_UNIT = 64;
+// A CTA's four warps take wh KV heads at a time, wp = 4 / wh warps each: with four heads no warp has to wait for another.  An
+// item is (sequence, wh KV heads, slab of query heads); its positions form units of 16 wp (8 wp for wide f32 rows), a tile for
+// each warp.  The work is cut evenly whatever the lengths: an item costs its units and ITEM_COST more for its beginning and
+// end, and worker w of G (one CTA each; G at most the whole cost U) takes what lies in [U w / G, U (w + 1) / G) of the batch
+// in order.  A worker finishes the items that lie inside its range; of an item that several workers share each leaves a
+// partial softmax (maximum, sum, weighted values) that paged_join_kernel folds in order.  A worker has at most two partial
+// items: slot 0 is one that began in an earlier worker, slot 1 one that begins here and goes on in the next.
+constexpr int MAX_CTAS_PER_SM = 4, MAX_UNIT = 64, ITEM_COST = 1;
 
 struct DecodeWs {
     int2* desc;      // (G): the split item that begins in worker w and its last worker; item -1: none
-    float* ml;       // (G, 2, rows, 2): maximum (log2 domain) and sum of a partial softmax
-    float* o;        // (G, 2, rows, dkm): its weighted values
+    float* ml;       // (G, 2, wh, rows, 2): maximum (log2 domain) and sum of a partial softmax
+    float* o;        // (G, 2, wh, rows, dkm): its weighted values
     float* lse2;     // (n_seq, n_head): log2 of the sum of exp, for the weights; or NULL
     float* scores;   // (n_seq, n_head, score_stride): scores in the log2 domain, for the weights; or NULL
     long long score_stride;
-    int rows, dkm;   // rows of an item and their pitch in the partial results
-    int slab_groups; // items per (sequence, KV head): larger groups of query heads than a pass serves are cut
+    int wh;
+    int rows, dkm;   // query heads of an item per KV head, and the pitch of the partial results
+    int slab_groups; // items per (sequence, wh KV heads): larger groups of query heads than a pass serves are cut
 };
 
-// position in the batch's order of units
+// an item's place in the batch and a tile of it
 struct UnitIter {
     int seq, hs, tile, n, tiles;
 };
 
-template <int UNIT>
-__device__ __forceinline__ void advance(UnitIter& it, const PagedView& c, const SeqView& s, int items_per_seq, int* flags)
+__device__ __forceinline__ void load_seq(UnitIter& it, const PagedView& c, const SeqView& s, int unit, int* flags)
 {
-    if (++it.tile < it.tiles) return;
+    it.n = paged_len(c, s, it.seq, flags);
+    it.tiles = (it.n + unit - 1) / unit;
+}
+// to the first tile of the next item
+__device__ __forceinline__ void next_item(UnitIter& it, const PagedView& c, const SeqView& s, int unit, int items_per_seq, int* flags)
+{
     it.tile = 0;
     if (++it.hs < items_per_seq) return;
     it.hs = 0;
     do {
-        it.n = paged_len(c, s, ++it.seq, flags);
-        it.tiles = (it.n + UNIT - 1) / UNIT;
+        ++it.seq;
+        load_seq(it, c, s, unit, flags);
     } while (it.tiles == 0 && it.seq + 1 < s.n_seq);
 }
 
-// Called by all 128 threads: this worker's units and the place of the first one.
-template <int UNIT>
-__device__ __forceinline__ bool find_work(const PagedView& c, const SeqView& s, int items_per_seq, UnitIter& it, long long& u0, long long& u1,
+// Called by all 128 threads: this worker's range of the cost and the place of its first unit; false if it has none.
+__device__ __forceinline__ bool find_work(const PagedView& c, const SeqView& s, int unit, int items_per_seq, UnitIter& it, long long& u0, long long& u1,
                                           long long& units, int& workers, int* flags)
 {
     __shared__ long long warp_sum[4], place;
     __shared__ int place_seq;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (s.n_seq + 127) / 128, first = min(s.n_seq, tid * per), last = min(s.n_seq, first + per);
+    auto cost = [&](int i) {
+        const int n = paged_len(c, s, i, flags);
+        return n ? (n + unit - 1) / unit + ITEM_COST : 0;
+    };
     long long mine = 0;
-    for (int i = first; i < last; ++i) mine += (paged_len(c, s, i, flags) + UNIT - 1) / UNIT;
+    for (int i = first; i < last; ++i) mine += cost(i);
     mine *= items_per_seq;
     long long incl = mine;
 #pragma unroll
@@ -95,7 +104,7 @@ __device__ __forceinline__ bool find_work(const PagedView& c, const SeqView& s, 
         int i = first;
         long long left = u0 - base;
         for (; i + 1 < last; ++i) {
-            const long long n = (long long)((paged_len(c, s, i, flags) + UNIT - 1) / UNIT) * items_per_seq;
+            const long long n = (long long)cost(i) * items_per_seq;
             if (left < n) break;
             left -= n;
         }
@@ -104,13 +113,17 @@ __device__ __forceinline__ bool find_work(const PagedView& c, const SeqView& s, 
     }
     __syncthreads();
     it.seq = place_seq;
-    it.n = paged_len(c, s, it.seq, flags);
-    it.tiles = (it.n + UNIT - 1) / UNIT;
-    it.hs = (int)(place / it.tiles);
-    it.tile = (int)(place % it.tiles);
+    load_seq(it, c, s, unit, flags);
+    it.hs = (int)(place / (it.tiles + ITEM_COST));
+    it.tile = (int)(place % (it.tiles + ITEM_COST));
+    if (it.tile >= it.tiles) {  // the range begins in what the end of an item costs
+        u0 += it.tiles + ITEM_COST - it.tile;
+        if (u0 >= u1) return false;
+        next_item(it, c, s, unit, items_per_seq, flags);
+    }
     return true;
 }
-// the worker that has unit u: the largest w with floor(units w / G) <= u
+// the worker that has position u of the cost: the largest w with floor(units w / G) <= u
 __device__ __forceinline__ int worker_of(long long u, long long units, int g) { return (int)(((u + 1) * g - 1) / units); }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void* p)
@@ -142,6 +155,13 @@ __device__ __forceinline__ uint32_t take_top(float& x, float& y)
     y = __fsub_rn(y, __uint_as_float(b & 0xffff0000u));
     return __byte_perm(a, b, 0x7632);
 }
+// 2^x for x <= 0 (results below the normal range are 0)
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ void cp16_zfill(void* smem, const void* gmem, bool valid)
 {
     const uint32_t sa = (uint32_t)__cvta_generic_to_shared(smem);
@@ -149,155 +169,268 @@ __device__ __forceinline__ void cp16_zfill(void* smem, const void* gmem, bool va
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(sa), "l"(gmem), "r"(sz) : "memory");
 }
 
+// the queries of the item that the issuing side has come to, into L1: they are read NST units later
+template <typename TQ>
+__device__ __forceinline__ void prefetch_queries(const PagedView& c, const DecodeArgs& a, const DecodeWs& ws, int seq, int hk, int row0)
+{
+    const TQ* q = (const TQ*)a.q + (long long)seq * a.q_stride + (long long)(hk * a.group + row0) * c.dk;
+    const int bytes = min(ws.rows, a.group - row0) * c.dk * (int)sizeof(TQ);
+    for (int b = (threadIdx.x & 31) * 128; b < bytes; b += 32 * 128) asm volatile("prefetch.global.L1 [%0];\n" ::"l"((const char*)q + b));
+}
+
+// the warps of a KV head (all of the CTA's where a head has more than one: they are at the same unit)
+__device__ __forceinline__ void sync_head(int wp)
+{
+    if (wp == 1)
+        __syncwarp();
+    else
+        __syncthreads();
+}
+
+// Folds the results that the wp warps of a KV head have parked (rows of STRIDE floats, then maximum and sum per row; warps
+// warp_stride floats apart) and writes them: outputs if the item is whole, a partial result otherwise.
+template <int DKM, int STRIDE, int ROWS, typename TQ>
+__device__ __forceinline__ void fold_warps(const float* parked, int warp_stride, int wp, const PagedView& c, const DecodeArgs& a, const DecodeWs& ws,
+                                           int seq, int hk, int row0, bool whole, int slot)
+{
+    const int rows = min(min(ROWS, ws.rows), a.group - row0), threads = 32 * wp, in_head = (threadIdx.x >> 5) / wp;
+    for (int p = threadIdx.x & (threads - 1); p < rows * (DKM / 4); p += threads) {
+        const int r = p / (DKM / 4), f = p % (DKM / 4) * 4;
+        float top = -INFINITY, sum = 0.0f;
+        for (int w = 0; w < wp; ++w) top = fmaxf(top, parked[w * warp_stride + ROWS * STRIDE + 2 * r]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int w = 0; w < wp; ++w) {
+            const float2 ml = *reinterpret_cast<const float2*>(parked + w * warp_stride + ROWS * STRIDE + 2 * r);
+            const float k = exp2f(ml.x - base);
+            const float4 y = *reinterpret_cast<const float4*>(parked + w * warp_stride + r * STRIDE + f);
+            sum = fmaf(ml.y, k, sum);
+            x.x = fmaf(y.x, k, x.x);
+            x.y = fmaf(y.y, k, x.y);
+            x.z = fmaf(y.z, k, x.z);
+            x.w = fmaf(y.w, k, x.w);
+        }
+        if (whole) {
+            const long long hq = (long long)seq * a.n_head + hk * a.group + row0 + r;
+            const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum), v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (f + i < c.dk) store_one((TQ*)a.out + hq * c.dk + f + i, v[i] * inv);
+            if (f == 0) {
+                const float z = sum == 0.0f ? -INFINITY : top + log2f(sum);
+                if (a.lse) a.lse[hq] = z * 0.693147180559945309f;
+                if (ws.lse2) ws.lse2[hq] = z;
+            }
+        } else {
+            const long long pr = (((long long)blockIdx.x * 2 + slot) * ws.wh + in_head) * ws.rows + r;
+            *reinterpret_cast<float4*>(ws.o + pr * ws.dkm + f) = x;
+            if (f == 0) *reinterpret_cast<float2*>(ws.ml + pr * 2) = make_float2(top, sum);
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ bf16 caches
-// What a configuration of the kernel needs.  KS: 16-feature steps of a row (dk padded with zeros in shared memory only);
-// NSLAB: slabs of 8 query heads that share one pass over the cache; PREC: f32 queries and outputs.
-template <int KS, int NSLAB, bool PREC>
+// Tensor cores multiply bf16, so queries and probabilities enter as bf16 pieces whose sum is the f32 value: two pieces keep 16
+// bits (bf16 queries are one), three keep 24 (PREC: f32 queries and outputs).  An m16 tile has room for the pieces of several
+// heads, so most come at no further multiplication: the thread that holds row g of an accumulator also holds row g + 8.
+//   HEADS 4:  leading pieces in rows 0-3, second in 8-11, third in 4-7 (the lanes 16 away)
+//   HEADS 8:  leading in rows 0-7, second in 8-15, third (if any) by a second multiplication
+//   HEADS 16: two slabs of the last kind that share the loaded tiles
+// KS: 16-feature steps of a row (dk padded with zeros, in shared memory only).
+template <int KS, int HEADS, bool PREC>
 struct MmaCfg {
-    static constexpr int DKM = KS * 16, LD = DKM + 8, TK = 16, UNIT = 4 * TK;
-    static constexpr bool REGQ = KS * NSLAB * (PREC ? 6 : 4) <= 64;  // query fragments in registers, else in shared memory
-    static constexpr int QROWS = REGQ ? 0 : NSLAB * (PREC ? 24 : 16);
-    static constexpr int STAGE = 2 * TK * LD;                        // elements of a warp's key and value tile
-    static constexpr int NST = KS > 8 || NSLAB == 2 ? 2 : 3;
-    static constexpr int MB_LD = DKM + 8;
-    static constexpr size_t SMEM = (size_t)4 * NST * STAGE * 2 + (size_t)QROWS * LD * 2 + 2 * 8 * MB_LD * 4 + 2 * 8 * 2 * 4;
-    static constexpr int CTAS = KS <= 8 ? 2 : 1;
+    static constexpr int NSLAB = HEADS == 16 ? 2 : 1, DKM = KS * 16, LD = DKM + 8, TK = 16;
+    static constexpr bool THIRD = PREC && HEADS > 4;                        // a second multiplication for the third pieces
+    static constexpr bool REGQ = KS * NSLAB * (THIRD ? 6 : 4) <= 64;        // query fragments in registers, else in shared memory
+    static constexpr int QS = NSLAB * (THIRD ? 24 : 16), QROWS = REGQ ? 0 : QS;
+    static constexpr int STAGE = 2 * TK * LD;                               // elements of a warp's key and value tile
+    static constexpr int NST = KS <= 8 && HEADS < 16 ? 3 : 2;
+    static constexpr int CTAS = KS == 4 ? (HEADS == 16 ? 2 : 4) : KS <= 8 ? 2 : 1;
+    // a warp's result of an item is parked over the tile that it has just used: rows of PARK floats, then maximum and sum
+    static constexpr int ROWS = 8 * NSLAB, PARK = DKM + (NSLAB == 1 ? 8 : 4);
+    static_assert((ROWS * PARK + 2 * ROWS) * 4 <= STAGE * 2, "a parked result fits in a stage");
+    static constexpr size_t SMEM = (size_t)4 * NST * STAGE * 2 + (size_t)(HEADS == 16 ? 1 : 4) * QROWS * LD * 2;  // queries: a copy per KV head of the CTA
 };
 
-template <int KS, int NSLAB, typename TQ>
-__global__ void __launch_bounds__(128, MmaCfg<KS, NSLAB, sizeof(TQ) == 4>::CTAS)
+template <int KS, int HEADS, typename TQ>
+__global__ void __launch_bounds__(128, MmaCfg<KS, HEADS, sizeof(TQ) == 4>::CTAS)
 paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, const DecodeWs ws, int* flags)
 {
     constexpr bool PREC = sizeof(TQ) == 4;
-    using C = MmaCfg<KS, NSLAB, PREC>;
-    constexpr int LD = C::LD, TK = C::TK, NST = C::NST, CH = 2 * KS, NT = 2 * KS;
+    using C = MmaCfg<KS, HEADS, PREC>;
+    constexpr int LD = C::LD, TK = C::TK, NST = C::NST, NSLAB = C::NSLAB, NT = 2 * KS;
+    constexpr bool SPREAD = PREC && HEADS == 4;  // the lanes 16 away hold the third pieces of the same head
+    // a load instruction covers RPI rows with CHP lanes each (2 KS of them with a 16-byte chunk of the padded row)
+    constexpr int CH = 2 * KS, CHP = KS <= 4 ? 8 : KS <= 8 ? 16 : 32, RPI = 32 / CHP;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     __nv_bfloat16* ring = reinterpret_cast<__nv_bfloat16*>(smem_raw) + (size_t)warp * NST * C::STAGE;
-    __nv_bfloat16* qs = reinterpret_cast<__nv_bfloat16*>(smem_raw) + (size_t)4 * NST * C::STAGE;
-    float* mb = reinterpret_cast<float*>(qs + (size_t)C::QROWS * LD);  // two parked partial results
-    float* mb_ml = mb + 2 * 8 * C::MB_LD;
+    __nv_bfloat16* qs = reinterpret_cast<__nv_bfloat16*>(smem_raw) + (size_t)4 * NST * C::STAGE + (size_t)(warp / (4 / ws.wh)) * C::QROWS * LD;
     pdl_wait();
     pdl_launch();
-    const int items_per_seq = c.heads * ws.slab_groups;
+    const int wp = 4 / ws.wh, unit = TK * wp, in_head = warp / wp, items_per_seq = c.heads / ws.wh * ws.slab_groups;
     UnitIter ct;
-    long long u, u1, units;
+    long long u_begin, u_end, units;
     int workers;
-    const bool work = find_work<C::UNIT>(c, s, items_per_seq, ct, u, u1, units, workers, flags);
+    const bool work = find_work(c, s, unit, items_per_seq, ct, u_begin, u_end, units, workers, flags);
     if (tid == 0) ws.desc[blockIdx.x] = make_int2(-1, -1);
     if (!work) return;
+    // cost left for the computing and for the issuing side, which runs NST units ahead
+    long long left = u_end - u_begin, to_issue = left;
 
-    const int chunks = c.pitch / 8;
     const char* kbase = (const char*)c.k;
     const char* vbase = (const char*)c.v;
-    const size_t row_bytes = (size_t)c.pitch * 2;
-    // the issuing side runs NST units ahead of the computing side; the page of its lane's row is loaded one unit ahead
+    const unsigned row_bytes = (unsigned)c.pitch * 2;
+    const int my_row = lane / CHP, my_ch = lane % CHP;
+    const bool my_live = my_ch < c.pitch / 8;
+    // Pages of a multiple of 16 positions: a tile lies in one page and its rows follow one another.  Otherwise each lane
+    // looks up the row of one position of the tile.
+    const bool whole_tiles = c.page % TK == 0;
+    const int my_pos = warp % wp * TK + (whole_tiles ? 0 : lane & 15);
+    const int col_step = unit / c.page, slot_step = unit % c.page;
     UnitIter it = ct;
-    long long iu = u;
-    int page_id = -1;
-    auto fetch_page = [&]() {
-        const int pos = it.tile * C::UNIT + warp * TK + (lane & 15);
-        if (iu < u1) page_id = pos < it.n ? s.table[(long long)it.seq * s.stride + pos / c.page] : -1;
-    };
-    fetch_page();
-    // which of the 16 positions of each tile under way exist (bit per position, the oldest tile lowest)
-    unsigned long long exist = 0;
+    int col = (it.tile * unit + my_pos) / c.page, slot_in_page = (it.tile * unit + my_pos) % c.page, page_id = -1;
+    int head = it.hs / ws.slab_groups * ws.wh + in_head;
+    const int32_t* table_row = s.table + (long long)it.seq * s.stride;
+    int ahead = it.n - it.tile * unit - my_pos;  // positions of the item from this lane's on
+    unsigned long long exist = 0;  // which of the 16 positions of each tile under way exist (a bit each, the oldest tile lowest)
+    if (ahead > 0) page_id = table_row[col];
     auto issue = [&](int stage, int age) {
-        unsigned mask = 0;
-        if (iu < u1) {
-            const int pos = it.tile * C::UNIT + warp * TK + (lane & 15);
+        if (to_issue > 0) {
+            unsigned mask = 0;
             int row = -1;
-            if (pos < it.n) {
-                row = (int)paged_row(page_id, c.n_pages, c.heads, c.page, it.hs / ws.slab_groups, pos % c.page);
-                if (row < 0) paged_flag(flags, PAGED_BAD_PAGE);
+            if (ahead > 0) {
+                if ((unsigned)page_id < (unsigned)c.n_pages)
+                    row = (page_id * c.heads + head) * c.page + slot_in_page;
+                else
+                    paged_flag(flags, PAGED_BAD_PAGE);
             }
-            mask = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
-            __nv_bfloat16* kt = ring + stage * C::STAGE;
+            __nv_bfloat16* kt = ring + stage * C::STAGE + my_row * LD + my_ch * 8;
             __nv_bfloat16* vt = kt + TK * LD;
+            if (whole_tiles) {
+                const int n = row >= 0 ? min(ahead, TK) : 0;
+                mask = (1u << n) - 1u;
+                const size_t off = n ? (size_t)(unsigned)row * row_bytes + my_row * row_bytes + my_ch * 16 : 0;
+                const char* kp = kbase + off;
+                const char* vp = vbase + off;
+                const int lim = my_live ? n - my_row : 0;  // row i * RPI + my_row exists: i * RPI < lim
+                if (CH == CHP || my_ch < CH)
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                const int idx = i * 32 + lane, r = idx / CH, ch = idx % CH;
-                const int src = __shfl_sync(0xffffffffu, row, r);
-                const bool ok = src >= 0 && ch < chunks;
-                const size_t off = ok ? (size_t)src * row_bytes + ch * 16 : 0;
-                cp16_zfill(kt + r * LD + ch * 8, kbase + off, ok);
-                cp16_zfill(vt + r * LD + ch * 8, vbase + off, ok);
+                    for (int i = 0; i < TK / RPI; ++i) {
+                        const bool ok = i * RPI < lim;
+                        cp16_zfill(kt + i * RPI * LD, ok ? kp : kbase, ok);
+                        cp16_zfill(vt + i * RPI * LD, ok ? vp : vbase, ok);
+                        kp += RPI * row_bytes;
+                        vp += RPI * row_bytes;
+                    }
+            } else {
+                mask = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+#pragma unroll
+                for (int i = 0; i < TK / RPI; ++i) {
+                    const int src = __shfl_sync(0xffffffffu, row, i * RPI + my_row);
+                    const bool ok = src >= 0 && my_live;
+                    const size_t off = ok ? (size_t)(unsigned)src * row_bytes + my_ch * 16 : 0;
+                    if (CH == CHP || my_ch < CH) {
+                        cp16_zfill(kt + i * RPI * LD, kbase + off, ok);
+                        cp16_zfill(vt + i * RPI * LD, vbase + off, ok);
+                    }
+                }
             }
-            if (++iu < u1) advance<C::UNIT>(it, c, s, items_per_seq, flags);
-            fetch_page();
+            exist |= (unsigned long long)mask << (16 * age);
+            --to_issue;
+            if (++it.tile == it.tiles) to_issue -= ITEM_COST;
+            if (to_issue > 0) {
+                if (it.tile < it.tiles) {
+                    ahead -= unit;
+                    col += col_step;
+                    slot_in_page += slot_step;
+                    if (slot_in_page >= c.page) {
+                        slot_in_page -= c.page;
+                        ++col;
+                    }
+                } else {
+                    next_item(it, c, s, unit, items_per_seq, flags);
+                    head = it.hs / ws.slab_groups * ws.wh + in_head;
+                    if (warp % wp == 0) prefetch_queries<TQ>(c, a, ws, it.seq, head, it.hs % ws.slab_groups * ws.rows);
+                    table_row = s.table + (long long)it.seq * s.stride;
+                    ahead = it.n - my_pos;
+                    col = my_pos / c.page;
+                    slot_in_page = my_pos % c.page;
+                }
+                if (ahead > 0) page_id = table_row[col];  // used by the next call
+            }
         }
-        exist |= (unsigned long long)mask << (16 * age);
         asm volatile("cp.async.commit_group;\n" ::);
     };
 #pragma unroll
     for (int i = 0; i < NST; ++i) issue(i, i);
 
     const float scale2 = a.scale * 1.44269504088896341f;
-    uint32_t qa[C::REGQ ? NSLAB : 1][C::REGQ ? KS : 1][4], qb[C::REGQ && PREC ? NSLAB : 1][C::REGQ && PREC ? KS : 1][2];
-    float o[NSLAB][NT][2], m[NSLAB], l[NSLAB];
+    uint32_t qa[C::REGQ ? NSLAB : 1][C::REGQ ? KS : 1][4], qb[C::REGQ && C::THIRD ? NSLAB : 1][C::REGQ && C::THIRD ? KS : 1][2];
+    // o[..][0..1]: row g, o[..][2..3]: row g + 8.  With f32 outputs row g (the leading pieces) is added in f32 after every tile:
+    // tensor cores truncate their sums, which only the small pieces can afford over a long context.
+    float o[NSLAB][NT][4], m[NSLAB], l[NSLAB];
     bool fresh = true, starts_here = false;
-    int stage = 0, slot = 0;
-    for (; u < u1; ++u) {
-        const int hk = ct.hs / ws.slab_groups, row0 = (ct.hs % ws.slab_groups) * (8 * NSLAB);  // first query head of the group here
-        if (fresh) {  // a new item: its queries, as bf16 pieces whose sum is the f32 value; row g the leading, row g + 8 the second
+    int stage = 0;
+    for (;; ) {
+        // this warp's KV head and the first query head of its group here
+        const int hk = ct.hs / ws.slab_groups * ws.wh + in_head, row0 = (ct.hs % ws.slab_groups) * HEADS;
+        if (fresh) {  // a new item: its queries
             fresh = false;
             starts_here = ct.tile == 0;
-            slot = starts_here ? 1 : 0;
-            if (!C::REGQ) __syncthreads();
+            if (!C::REGQ) sync_head(wp);
 #pragma unroll
             for (int sl = 0; sl < NSLAB; ++sl) {
                 m[sl] = -INFINITY;
                 l[sl] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < NT; ++i) o[sl][i][0] = o[sl][i][1] = 0.0f;
-                const int gi = row0 + sl * 8 + g;
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[sl][i][j] = 0.0f;
+                const int gi = row0 + (HEADS == 4 ? g & 3 : sl * 8 + g);
                 const TQ* q = (const TQ*)a.q + (long long)ct.seq * a.q_stride + (long long)(hk * a.group + gi) * c.dk;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    if (!C::REGQ && (ks & 3) != warp) continue;
+                    if (!C::REGQ && (ks & (wp - 1)) != warp % wp) continue;
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
-                        const int col = ks * 16 + hf * 8 + 2 * t4;
-                        const float2 x = gi < a.group && col < c.dk ? load_pair(q + col) : make_float2(0.0f, 0.0f);
-                        const uint32_t hi = pack_rn(x.x, x.y);
-                        uint32_t lo = 0, lo2 = 0;
+                        const int f = ks * 16 + hf * 8 + 2 * t4;
+                        const float2 x = gi < a.group && f < c.dk ? load_pair(q + f) : make_float2(0.0f, 0.0f);
+                        uint32_t hi = pack_rn(x.x, x.y), lo = 0, lo2 = 0;
                         if (PREC) {
                             const float r0 = __fsub_rn(x.x, __uint_as_float(hi << 16)), r1 = __fsub_rn(x.y, __uint_as_float(hi & 0xffff0000u));
                             lo = pack_rn(r0, r1);
                             lo2 = pack_rn(__fsub_rn(r0, __uint_as_float(lo << 16)), __fsub_rn(r1, __uint_as_float(lo & 0xffff0000u)));
                         }
+                        if (HEADS == 4 && g >= 4) {
+                            hi = lo2;
+                            lo = 0;
+                        }
                         if constexpr (C::REGQ) {
                             qa[sl][ks][2 * hf] = hi;
                             qa[sl][ks][2 * hf + 1] = lo;
-                            if constexpr (PREC) qb[sl][ks][hf] = lo2;
+                            if constexpr (C::THIRD) qb[sl][ks][hf] = lo2;
                         } else {
-                            __nv_bfloat16* dst = qs + (size_t)sl * (PREC ? 24 : 16) * LD + col;
+                            __nv_bfloat16* dst = qs + (size_t)sl * (C::QS / NSLAB) * LD + f;
                             *reinterpret_cast<uint32_t*>(dst + g * LD) = hi;
                             *reinterpret_cast<uint32_t*>(dst + (8 + g) * LD) = lo;
-                            if (PREC) *reinterpret_cast<uint32_t*>(dst + (16 + g) * LD) = lo2;
+                            if (C::THIRD) *reinterpret_cast<uint32_t*>(dst + (16 + g) * LD) = lo2;
                         }
                     }
                 }
             }
-            if (!C::REGQ) __syncthreads();
+            if (!C::REGQ) sync_head(wp);
         }
         asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 1) : "memory");
         __syncwarp();
         const __nv_bfloat16* kt = ring + stage * C::STAGE;
         const __nv_bfloat16* vt = kt + TK * LD;
-        const int t0 = ct.tile * C::UNIT + warp * TK;
         const unsigned live = (unsigned)exist & 0xffffu;
         exist >>= 16;
-        // scores of 16 positions: n-tile j holds positions t0 + 8 j + 2 t4 + {0, 1} of head g
+        // scores of 16 positions: n-tile j holds positions 8 j + 2 t4 + {0, 1} of the tile, of the thread's head
         float x[NSLAB][2][2];
         {
-            float acc[NSLAB][2][4], acc2[NSLAB][2][4];
-#pragma unroll
-            for (int sl = 0; sl < NSLAB; ++sl)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[sl][j][i] = acc2[sl][j][i] = 0.0f;
+            float acc[NSLAB][2][2][4];  // two sums per n-tile (even and odd steps) halve the chain of dependent multiplications
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 uint32_t b[4];
@@ -308,23 +441,24 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
                     if constexpr (C::REGQ) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) f[i] = qa[sl][ks][i];
-                        if constexpr (PREC) {
+                        if constexpr (C::THIRD) {
                             f2[0] = qb[sl][ks][0];
                             f2[1] = qb[sl][ks][1];
                         }
                     } else {
-                        const __nv_bfloat16* src = qs + (size_t)sl * (PREC ? 24 : 16) * LD + ks * 16;
+                        const __nv_bfloat16* src = qs + (size_t)sl * (C::QS / NSLAB) * LD + ks * 16;
                         ldsm4(f, src + ((lane & 7) + 8 * ((lane >> 3) & 1)) * LD + 8 * (lane >> 4));
-                        if constexpr (PREC) {
+                        if constexpr (C::THIRD) {
                             f2[0] = *reinterpret_cast<const uint32_t*>(src + (16 + g) * LD + 2 * t4);
                             f2[1] = *reinterpret_cast<const uint32_t*>(src + (16 + g) * LD + 8 + 2 * t4);
                         }
                     }
-                    mma16816(acc[sl][0], f[0], f[1], f[2], f[3], b[0], b[1]);
-                    mma16816(acc[sl][1], f[0], f[1], f[2], f[3], b[2], b[3]);
-                    if constexpr (PREC) {
-                        mma16816(acc2[sl][0], f2[0], 0u, f2[1], 0u, b[0], b[1]);
-                        mma16816(acc2[sl][1], f2[0], 0u, f2[1], 0u, b[2], b[3]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float(&d)[4] = acc[sl][j][ks & 1];
+                        if (ks < 2) d[0] = d[1] = d[2] = d[3] = 0.0f;
+                        mma16816(d, f[0], f[1], f[2], f[3], b[2 * j], b[2 * j + 1]);
+                        if constexpr (C::THIRD) mma16816(d, f2[0], 0u, f2[1], 0u, b[2 * j], b[2 * j + 1]);
                     }
                 }
             }
@@ -334,16 +468,27 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float y = __fadd_rn(acc[sl][j][i], acc[sl][j][2 + i]);
-                        if constexpr (PREC) y = __fadd_rn(y, acc2[sl][j][i]);
-                        x[sl][j][i] = (live >> (8 * j + 2 * t4 + i)) & 1u ? __fmul_rn(y, scale2) : -INFINITY;
+                        float y = __fadd_rn(acc[sl][j][0][i], acc[sl][j][1][i]);
+                        if (PREC) y = __fadd_rn(y, __fadd_rn(acc[sl][j][0][2 + i], acc[sl][j][1][2 + i]));
+                        if (SPREAD) y = __fadd_rn(y, __shfl_xor_sync(0xffffffffu, y, 16));
+                        x[sl][j][i] = __fmul_rn(y, scale2);
                     }
+            if (live != 0xffffu)
+#pragma unroll
+                for (int sl = 0; sl < NSLAB; ++sl)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            if (!((live >> (8 * j + 2 * t4 + i)) & 1u)) x[sl][j][i] = -INFINITY;
         }
         float corr[NSLAB];
+        bool moved = false;
 #pragma unroll
         for (int sl = 0; sl < NSLAB; ++sl) {
-            if (ws.scores && row0 + sl * 8 + g < a.group) {
-                float* dst = ws.scores + ((long long)ct.seq * a.n_head + hk * a.group + row0 + sl * 8 + g) * ws.score_stride + t0 + 2 * t4;
+            const int gi = row0 + (HEADS == 4 ? g : sl * 8 + g);
+            if (ws.scores && gi < a.group && (HEADS != 4 || g < 4)) {
+                float* dst = ws.scores + ((long long)ct.seq * a.n_head + hk * a.group + gi) * ws.score_stride + ct.tile * unit + warp % wp * TK + 2 * t4;
                 *reinterpret_cast<float2*>(dst) = make_float2(x[sl][0][0], x[sl][0][1]);
                 *reinterpret_cast<float2*>(dst + 8) = make_float2(x[sl][1][0], x[sl][1][1]);
             }
@@ -351,18 +496,27 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(m[sl], fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)));
             const float base = top == -INFINITY ? 0.0f : top;  // nothing seen yet: every exponential is 0
-            corr[sl] = exp2f(m[sl] - base);
+            corr[sl] = exp2_fast(m[sl] - base);
+            moved |= top != m[sl];
             m[sl] = top;
             l[sl] *= corr[sl];
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    x[sl][j][i] = exp2f(x[sl][j][i] - base);
+                    x[sl][j][i] = exp2_fast(x[sl][j][i] - base);
                     l[sl] += x[sl][j][i];
                 }
         }
-        // o = o * corr + p . v, p as bf16 pieces (16 bits of it, 24 for f32 outputs) in rows g and g + 8
+        // o = o * corr + p . v; the sums that stay in the tensor cores are rescaled when a maximum has moved
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int sl = 0; sl < NSLAB; ++sl)
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[sl][i][j] *= corr[sl];
+        }
         uint32_t pa[NSLAB][4], pb[NSLAB][2];
 #pragma unroll
         for (int sl = 0; sl < NSLAB; ++sl)
@@ -373,6 +527,10 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
                 if constexpr (PREC) {
                     pa[sl][2 * j + 1] = take_top(p0, p1);
                     pb[sl][j] = pack_rn(p0, p1);
+                    if (SPREAD && g >= 4) {
+                        pa[sl][2 * j] = pb[sl][j];
+                        pa[sl][2 * j + 1] = 0u;
+                    }
                 } else {
                     pa[sl][2 * j + 1] = pack_rn(p0, p1);
                 }
@@ -385,84 +543,57 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
             for (int sl = 0; sl < NSLAB; ++sl)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma16816(acc, pa[sl][0], pa[sl][1], pa[sl][2], pa[sl][3], b[2 * j], b[2 * j + 1]);
-                    if constexpr (PREC) mma16816(acc, pb[sl][0], 0u, pb[sl][1], 0u, b[2 * j], b[2 * j + 1]);
-                    o[sl][2 * np + j][0] = fmaf(o[sl][2 * np + j][0], corr[sl], __fadd_rn(acc[0], acc[2]));
-                    o[sl][2 * np + j][1] = fmaf(o[sl][2 * np + j][1], corr[sl], __fadd_rn(acc[1], acc[3]));
+                    float(&d)[4] = o[sl][2 * np + j];
+                    if constexpr (PREC) {
+                        float y[4] = {0.0f, 0.0f, d[2], d[3]};
+                        mma16816(y, pa[sl][0], pa[sl][1], pa[sl][2], pa[sl][3], b[2 * j], b[2 * j + 1]);
+                        if constexpr (C::THIRD) mma16816(y, pb[sl][0], 0u, pb[sl][1], 0u, b[2 * j], b[2 * j + 1]);
+                        d[0] = __fadd_rn(d[0], y[0]);
+                        d[1] = __fadd_rn(d[1], y[1]);
+                        d[2] = y[2];
+                        d[3] = y[3];
+                    } else {
+                        mma16816(d, pa[sl][0], pa[sl][1], pa[sl][2], pa[sl][3], b[2 * j], b[2 * j + 1]);
+                    }
                 }
         }
         __syncwarp();
-        issue(stage, NST - 1);
-        stage = stage + 1 == NST ? 0 : stage + 1;
-
         const bool ends = ct.tile + 1 == ct.tiles;
-        if (ends || u + 1 == u1) {  // fold the four warps' results; warp 0 writes
+        left -= ends ? 1 + ITEM_COST : 1;
+        const bool last = left <= 0;
+        if (ends || last) {  // fold the four warps' results
             const bool whole = starts_here && ends;
             if (tid == 0 && starts_here && !ends)
-                ws.desc[blockIdx.x] = make_int2(ct.seq * items_per_seq + ct.hs, worker_of(u + (ct.tiles - 1 - ct.tile), units, workers));
+                ws.desc[blockIdx.x] = make_int2(ct.seq * items_per_seq + ct.hs, worker_of(u_end - 1 + (ct.tiles - 1 - ct.tile), units, workers));
+            float* park = reinterpret_cast<float*>(ring + stage * C::STAGE);
 #pragma unroll
             for (int sl = 0; sl < NSLAB; ++sl) {
-                float ls = l[sl], ms = m[sl];
+                float ls = l[sl];
                 ls += __shfl_xor_sync(0xffffffffu, ls, 1);
                 ls += __shfl_xor_sync(0xffffffffu, ls, 2);
-                auto park = [&](int buf) {
-                    float* dst = mb + (buf * 8 + g) * C::MB_LD + 2 * t4;
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[sl][i][0], o[sl][i][1]);
-                    if (t4 == 0) *reinterpret_cast<float2*>(mb_ml + (buf * 8 + g) * 2) = make_float2(ms, ls);
-                };
-                auto fold = [&](int buf) {
-                    const float* src = mb + (buf * 8 + g) * C::MB_LD + 2 * t4;
-                    const float2 ml = *reinterpret_cast<const float2*>(mb_ml + (buf * 8 + g) * 2);
-                    const float top = fmaxf(ms, ml.x), base = top == -INFINITY ? 0.0f : top;
-                    const float ca = exp2f(ms - base), cb = exp2f(ml.x - base);
-                    ms = top;
-                    ls = fmaf(ls, ca, ml.y * cb);
+                for (int i = 0; i < NT; ++i)
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        const float2 y = *reinterpret_cast<const float2*>(src + i * 8);
-                        o[sl][i][0] = fmaf(o[sl][i][0], ca, y.x * cb);
-                        o[sl][i][1] = fmaf(o[sl][i][1], ca, y.y * cb);
+                    for (int j = 0; j < 2; ++j) {
+                        o[sl][i][j] += o[sl][i][2 + j];
+                        if (SPREAD) o[sl][i][j] += __shfl_xor_sync(0xffffffffu, o[sl][i][j], 16);
                     }
-                };
-                __syncthreads();
-                if (warp >= 2) park(warp - 2);
-                __syncthreads();
-                if (warp < 2) fold(warp);
-                __syncthreads();
-                if (warp == 1) park(0);
-                __syncthreads();
-                if (warp == 0) {
-                    fold(0);
-                    const int gi = row0 + sl * 8 + g;
-                    if (whole && gi < a.group) {
-                        const long long hq = (long long)ct.seq * a.n_head + hk * a.group + gi;
-                        const float inv = ls == 0.0f ? 0.0f : __fdiv_rn(1.0f, ls);
-                        TQ* dst = (TQ*)a.out + hq * c.dk + 2 * t4;
+                if (row0 + sl * 8 + g >= a.group || (HEADS == 4 && g >= 4)) continue;
+                float* dst = park + (sl * 8 + g) * C::PARK + 2 * t4;
 #pragma unroll
-                        for (int i = 0; i < NT; ++i)
-                            if (i * 8 + 2 * t4 < c.dk) {
-                                store_one(dst + i * 8, o[sl][i][0] * inv);
-                                store_one(dst + i * 8 + 1, o[sl][i][1] * inv);
-                            }
-                        if (t4 == 0) {
-                            const float z = ls == 0.0f ? -INFINITY : ms + log2f(ls);
-                            if (a.lse) a.lse[hq] = z * 0.693147180559945309f;
-                            if (ws.lse2) ws.lse2[hq] = z;
-                        }
-                    } else if (!whole) {
-                        const long long r = ((long long)blockIdx.x * 2 + slot) * ws.rows + sl * 8 + g;
-                        float* dst = ws.o + r * ws.dkm + 2 * t4;
-#pragma unroll
-                        for (int i = 0; i < NT; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[sl][i][0], o[sl][i][1]);
-                        if (t4 == 0) *reinterpret_cast<float2*>(ws.ml + r * 2) = make_float2(ms, ls);
-                    }
-                }
+                for (int i = 0; i < NT; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[sl][i][0], o[sl][i][1]);
+                if (t4 == 0) *reinterpret_cast<float2*>(park + C::ROWS * C::PARK + (sl * 8 + g) * 2) = make_float2(m[sl], ls);
             }
+            sync_head(wp);
+            fold_warps<C::DKM, C::PARK, C::ROWS, TQ>(reinterpret_cast<const float*>(smem_raw) + (in_head * wp * NST + stage) * (C::STAGE / 2),
+                                                     NST * (C::STAGE / 2), wp, c, a, ws, ct.seq, hk, row0, whole, starts_here ? 1 : 0);
+            sync_head(wp);
             fresh = true;
         }
-        if (u + 1 < u1) advance<C::UNIT>(ct, c, s, items_per_seq, flags);
+        if (last) break;
+        issue(stage, NST - 1);
+        stage = stage + 1 == NST ? 0 : stage + 1;
+        if (++ct.tile == ct.tiles) next_item(ct, c, s, unit, items_per_seq, flags);
     }
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
 }
@@ -472,14 +603,13 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
 // NFI vectors of four features each; ROWS query heads (at most 8) share a pass.
 template <int FL, int NFI, int ROWS>
 struct FmaCfg {
-    static constexpr int TK = NFI == 2 ? 8 : 16, UNIT = 4 * TK, LPK = 32 / TK, NST = NFI == 2 ? 2 : 3, DKM = FL * 4 * NFI;
-    static constexpr int MB = ROWS * DKM + (2 * ROWS + 3) / 4 * 4;  // a parked partial result: values, then maximum and sum per row
+    static constexpr int TK = NFI == 2 ? 8 : 16, LPK = 32 / TK, NST = NFI == 2 || (FL == 16 && ROWS >= 4) ? 2 : 3, DKM = FL * 4 * NFI;
     // pitch of a row in shared memory: 4 * LPK floats beyond a multiple of 32, so that the keys of a quarter warp, LPK lanes
     // each, fall on different banks
     static __host__ __device__ constexpr int ld(int pitch) { return pitch + (4 * LPK + 32 - pitch % 32) % 32; }
     static __host__ __device__ constexpr size_t smem(int pitch)
     {
-        return ((size_t)4 * NST * 2 * TK * ld(pitch) + (size_t)ROWS * ld(pitch) + 4 * TK * ROWS + (size_t)2 * MB) * sizeof(float);
+        return ((size_t)4 * NST * 2 * TK * ld(pitch) + (size_t)4 * ROWS * ld(pitch) + 4 * TK * ROWS) * sizeof(float);
     }
 };
 
@@ -492,61 +622,81 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
     extern __shared__ __align__(16) float smem_f[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ld = C::ld(c.pitch), stage_len = 2 * TK * ld;
     float* ring = smem_f + (size_t)warp * NST * stage_len;
-    float* qs = smem_f + (size_t)4 * NST * stage_len;
-    float* ps = qs + (size_t)ROWS * ld + warp * TK * ROWS;  // this warp's probabilities, (position, row)
-    float* mb = qs + (size_t)ROWS * ld + 4 * TK * ROWS;     // two parked partial results
     pdl_wait();
     pdl_launch();
-    const int items_per_seq = c.heads * ws.slab_groups;
+    const int wp = 4 / ws.wh, unit = TK * wp, in_head = warp / wp, items_per_seq = c.heads / ws.wh * ws.slab_groups;
+    float* qs = smem_f + (size_t)4 * NST * stage_len + (size_t)in_head * ROWS * ld;  // one copy per KV head of the CTA
+    float* ps = smem_f + (size_t)4 * NST * stage_len + (size_t)ws.wh * ROWS * ld + warp * TK * ROWS;  // this warp's probabilities, (position, row)
     UnitIter ct;
-    long long u, u1, units;
+    long long u_begin, u_end, units;
     int workers;
-    const bool work = find_work<C::UNIT>(c, s, items_per_seq, ct, u, u1, units, workers, flags);
+    const bool work = find_work(c, s, unit, items_per_seq, ct, u_begin, u_end, units, workers, flags);
     if (tid == 0) ws.desc[blockIdx.x] = make_int2(-1, -1);
     if (!work) return;
+    long long left = u_end - u_begin, to_issue = left;
 
     const int chunks = c.pitch / 4, key = lane / LPK, sub = lane % LPK;
     const float* kbase = (const float*)c.k;
     const float* vbase = (const float*)c.v;
+    // as in the bf16 kernel; each lane looks up the row of one position of the tile
+    const int my_pos = warp % wp * TK + lane % TK, col_step = unit / c.page, slot_step = unit % c.page;
     UnitIter it = ct;
-    long long iu = u;
-    int page_id = -1;
-    auto fetch_page = [&]() {
-        const int pos = it.tile * C::UNIT + warp * TK + lane % TK;
-        if (iu < u1) page_id = pos < it.n ? s.table[(long long)it.seq * s.stride + pos / c.page] : -1;
-    };
-    fetch_page();
-    unsigned long long exist = 0;  // as in the bf16 kernel
+    int col = (it.tile * unit + my_pos) / c.page, slot_in_page = (it.tile * unit + my_pos) % c.page, page_id = -1;
+    int head = it.hs / ws.slab_groups * ws.wh + in_head;
+    const int32_t* table_row = s.table + (long long)it.seq * s.stride;
+    int ahead = it.n - it.tile * unit - my_pos;
+    unsigned long long exist = 0;
+    if (ahead > 0) page_id = table_row[col];
     auto issue = [&](int stage, int age) {
-        unsigned mask = 0;
-        if (iu < u1) {
-            const int pos = it.tile * C::UNIT + warp * TK + lane % TK;
+        if (to_issue > 0) {
             int row = -1;
-            if (pos < it.n) {
-                row = (int)paged_row(page_id, c.n_pages, c.heads, c.page, it.hs / ws.slab_groups, pos % c.page);
-                if (row < 0) paged_flag(flags, PAGED_BAD_PAGE);
+            if (ahead > 0) {
+                if ((unsigned)page_id < (unsigned)c.n_pages)
+                    row = (page_id * c.heads + head) * c.page + slot_in_page;
+                else
+                    paged_flag(flags, PAGED_BAD_PAGE);
             }
-            mask = __ballot_sync(0xffffffffu, row >= 0) & ((1u << TK) - 1u);
+            const unsigned mask = __ballot_sync(0xffffffffu, row >= 0) & ((1u << TK) - 1u);
             float* kt = ring + stage * stage_len;
             float* vt = kt + TK * ld;
 #pragma unroll
             for (int i = 0; i < TK / RPI; ++i) {
                 const int r = i * RPI + lane / FL;
                 const int src = __shfl_sync(0xffffffffu, row, r);
+                const size_t off = src >= 0 ? (size_t)(unsigned)src * c.pitch + lane % FL * 4 : 0;
 #pragma unroll
                 for (int j = 0; j < NFI; ++j) {
                     const int ch = lane % FL + FL * j;
                     if (ch < chunks) {
-                        const size_t off = src >= 0 ? (size_t)src * c.pitch + ch * 4 : 0;
-                        cp16_zfill(kt + r * ld + ch * 4, kbase + off, src >= 0);
-                        cp16_zfill(vt + r * ld + ch * 4, vbase + off, src >= 0);
+                        cp16_zfill(kt + r * ld + ch * 4, src >= 0 ? kbase + off + FL * 4 * j : kbase, src >= 0);
+                        cp16_zfill(vt + r * ld + ch * 4, src >= 0 ? vbase + off + FL * 4 * j : vbase, src >= 0);
                     }
                 }
             }
-            if (++iu < u1) advance<C::UNIT>(it, c, s, items_per_seq, flags);
-            fetch_page();
+            exist |= (unsigned long long)mask << (16 * age);
+            --to_issue;
+            if (++it.tile == it.tiles) to_issue -= ITEM_COST;
+            if (to_issue > 0) {
+                if (it.tile < it.tiles) {
+                    ahead -= unit;
+                    col += col_step;
+                    slot_in_page += slot_step;
+                    if (slot_in_page >= c.page) {
+                        slot_in_page -= c.page;
+                        ++col;
+                    }
+                } else {
+                    next_item(it, c, s, unit, items_per_seq, flags);
+                    head = it.hs / ws.slab_groups * ws.wh + in_head;
+                    if (warp % wp == 0) prefetch_queries<TQ>(c, a, ws, it.seq, head, it.hs % ws.slab_groups * ws.rows);
+                    table_row = s.table + (long long)it.seq * s.stride;
+                    ahead = it.n - my_pos;
+                    col = my_pos / c.page;
+                    slot_in_page = my_pos % c.page;
+                }
+                if (ahead > 0) page_id = table_row[col];
+            }
         }
-        exist |= (unsigned long long)mask << (16 * age);
         asm volatile("cp.async.commit_group;\n" ::);
     };
 #pragma unroll
@@ -556,20 +706,19 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
     float4 o[ROWS][NFI];
     float m[ROWS], l[ROWS];  // l: this lane's share
     bool fresh = true, starts_here = false;
-    int stage = 0, slot = 0;
-    for (; u < u1; ++u) {
-        const int hk = ct.hs / ws.slab_groups, row0 = (ct.hs % ws.slab_groups) * ROWS;
+    int stage = 0;
+    for (;;) {
+        const int hk = ct.hs / ws.slab_groups * ws.wh + in_head, row0 = (ct.hs % ws.slab_groups) * ROWS;
         if (fresh) {
             fresh = false;
             starts_here = ct.tile == 0;
-            slot = starts_here ? 1 : 0;
             const TQ* q = (const TQ*)a.q + (long long)ct.seq * a.q_stride + (long long)(hk * a.group + row0) * c.dk;
-            __syncthreads();
-            for (int i = tid; i < ROWS * c.pitch; i += 128) {
-                const int r = i / c.pitch, f = i % c.pitch;
-                qs[r * ld + f] = row0 + r < a.group && f < c.dk ? load_one(q + r * c.dk + f) : 0.0f;
-            }
-            __syncthreads();
+            sync_head(wp);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+                for (int f = tid & (32 * wp - 1); f < c.pitch; f += 32 * wp)
+                    qs[r * ld + f] = row0 + r < a.group && f < c.dk ? load_one(q + r * c.dk + f) : 0.0f;
+            sync_head(wp);
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 m[r] = -INFINITY;
@@ -582,7 +731,7 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
         __syncwarp();
         const float* kt = ring + stage * stage_len;
         const float* vt = kt + TK * ld;
-        const int t0 = ct.tile * C::UNIT + warp * TK;
+        const int t0 = ct.tile * unit + warp % wp * TK;
         const unsigned live = (unsigned)exist & 0xffffu;
         exist >>= 16;
         // scores: LPK lanes per position, every LPK-th vector of the row each
@@ -647,14 +796,13 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
             }
         }
         __syncwarp();
-        issue(stage, NST - 1);
-        stage = stage + 1 == NST ? 0 : stage + 1;
-
         const bool ends = ct.tile + 1 == ct.tiles;
-        if (ends || u + 1 == u1) {  // fold the lanes' and the warps' results; warp 0 writes
+        left -= ends ? 1 + ITEM_COST : 1;
+        const bool last = left <= 0;
+        if (ends || last) {  // fold the lanes' and the warps' results
             const bool whole = starts_here && ends;
             if (tid == 0 && starts_here && !ends)
-                ws.desc[blockIdx.x] = make_int2(ct.seq * items_per_seq + ct.hs, worker_of(u + (ct.tiles - 1 - ct.tile), units, workers));
+                ws.desc[blockIdx.x] = make_int2(ct.seq * items_per_seq + ct.hs, worker_of(u_end - 1 + (ct.tiles - 1 - ct.tile), units, workers));
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 l[r] = warp_sum(l[r]) * (1.0f / LPK);
@@ -668,79 +816,27 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
                         o[r][j].w += __shfl_xor_sync(0xffffffffu, o[r][j].w, d);
                     }
             }
-            auto park = [&](float* buf) {
+            float* park = ring + stage * stage_len;  // over the tile that was just used
 #pragma unroll
-                for (int r = 0; r < ROWS; ++r) {
-                    if (lane < FL)
+            for (int r = 0; r < ROWS; ++r) {
+                if (lane < FL)
 #pragma unroll
-                        for (int j = 0; j < NFI; ++j) *reinterpret_cast<float4*>(buf + r * C::DKM + (lane + FL * j) * 4) = o[r][j];
-                    if (lane == 0) {
-                        buf[ROWS * C::DKM + 2 * r] = m[r];
-                        buf[ROWS * C::DKM + 2 * r + 1] = l[r];
-                    }
-                }
-            };
-            auto fold = [&](const float* buf) {
-#pragma unroll
-                for (int r = 0; r < ROWS; ++r) {
-                    const float mo = buf[ROWS * C::DKM + 2 * r], lo = buf[ROWS * C::DKM + 2 * r + 1];
-                    const float top = fmaxf(m[r], mo), base = top == -INFINITY ? 0.0f : top;
-                    const float ca = exp2f(m[r] - base), cb = exp2f(mo - base);
-                    m[r] = top;
-                    l[r] = fmaf(l[r], ca, lo * cb);
-#pragma unroll
-                    for (int j = 0; j < NFI; ++j) {
-                        const float4 y = *reinterpret_cast<const float4*>(buf + r * C::DKM + (lane % FL + FL * j) * 4);
-                        o[r][j].x = fmaf(o[r][j].x, ca, y.x * cb);
-                        o[r][j].y = fmaf(o[r][j].y, ca, y.y * cb);
-                        o[r][j].z = fmaf(o[r][j].z, ca, y.z * cb);
-                        o[r][j].w = fmaf(o[r][j].w, ca, y.w * cb);
-                    }
-                }
-            };
-            __syncthreads();
-            if (warp >= 2) park(mb + (warp - 2) * C::MB);
-            __syncthreads();
-            if (warp < 2) fold(mb + warp * C::MB);
-            __syncthreads();
-            if (warp == 1) park(mb);
-            __syncthreads();
-            if (warp == 0) {
-                fold(mb);
-#pragma unroll
-                for (int r = 0; r < ROWS; ++r) {
-                    if (row0 + r >= a.group) continue;
-                    const long long hq = (long long)ct.seq * a.n_head + hk * a.group + row0 + r;
-                    const long long pr = ((long long)blockIdx.x * 2 + slot) * ws.rows + r;
-                    const float inv = l[r] == 0.0f ? 0.0f : __fdiv_rn(1.0f, l[r]);
-#pragma unroll
-                    for (int j = 0; j < NFI; ++j) {
-                        const int f = (lane + FL * j) * 4;
-                        if (lane >= FL) continue;
-                        if (!whole) {
-                            *reinterpret_cast<float4*>(ws.o + pr * ws.dkm + f) = o[r][j];
-                        } else {
-                            const float v[4] = {o[r][j].x, o[r][j].y, o[r][j].z, o[r][j].w};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (f + i < c.dk) store_one((TQ*)a.out + hq * c.dk + f + i, v[i] * inv);
-                        }
-                    }
-                    if (lane == 0) {
-                        if (!whole) {
-                            ws.ml[pr * 2] = m[r];
-                            ws.ml[pr * 2 + 1] = l[r];
-                        } else {
-                            const float z = l[r] == 0.0f ? -INFINITY : m[r] + log2f(l[r]);
-                            if (a.lse) a.lse[hq] = z * 0.693147180559945309f;
-                            if (ws.lse2) ws.lse2[hq] = z;
-                        }
-                    }
+                    for (int j = 0; j < NFI; ++j) *reinterpret_cast<float4*>(park + r * C::DKM + (lane + FL * j) * 4) = o[r][j];
+                if (lane == 0) {
+                    park[ROWS * C::DKM + 2 * r] = m[r];
+                    park[ROWS * C::DKM + 2 * r + 1] = l[r];
                 }
             }
+            sync_head(wp);
+            fold_warps<C::DKM, C::DKM, ROWS, TQ>(smem_f + (in_head * wp * NST + stage) * stage_len, NST * stage_len, wp, c, a, ws, ct.seq, hk, row0, whole,
+                                                 starts_here ? 1 : 0);
+            sync_head(wp);
             fresh = true;
         }
-        if (u + 1 < u1) advance<C::UNIT>(ct, c, s, items_per_seq, flags);
+        if (last) break;
+        issue(stage, NST - 1);
+        stage = stage + 1 == NST ? 0 : stage + 1;
+        if (++ct.tile == ct.tiles) next_item(ct, c, s, unit, items_per_seq, flags);
     }
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
 }
@@ -764,11 +860,11 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedView c, cons
             }
     const int2 d = ws.desc[w0];
     if (d.x < 0) return;
-    const int items_per_seq = c.heads * ws.slab_groups, seq = d.x / items_per_seq, hs = d.x % items_per_seq;
-    const int gi = hs % ws.slab_groups * ws.rows + row, n = d.y - w0 + 1;
+    const int items_per_seq = c.heads / ws.wh * ws.slab_groups, seq = d.x / items_per_seq, hs = d.x % items_per_seq;
+    const int gi = hs % ws.slab_groups * ws.rows + row % ws.rows, hk = hs / ws.slab_groups * ws.wh + row / ws.rows, n = d.y - w0 + 1;
     if (gi >= a.group) return;
     // the first worker's partial result is in its slot 1, the others' in slot 0
-    auto at = [&](int i) { return ((long long)(w0 + i) * 2 + (i == 0 ? 1 : 0)) * ws.rows + row; };
+    auto at = [&](int i) { return ((long long)(w0 + i) * 2 + (i == 0 ? 1 : 0)) * ws.wh * ws.rows + row; };
     float top = -INFINITY;
     for (int i = tid; i < n; i += 128) top = fmaxf(top, ws.ml[at(i) * 2]);
     top = warp_max(top);
@@ -804,7 +900,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedView c, cons
     float4* sums = reinterpret_cast<float4*>(wgt);
     sums[tid] = acc;
     __syncthreads();
-    const long long hq = (long long)seq * a.n_head + hs / ws.slab_groups * a.group + gi;
+    const long long hq = (long long)seq * a.n_head + hk * a.group + gi;
     if (part == 0) {
         for (int p = 1; p < parts; ++p) {
             const float4 y = sums[p * lanes + f];
@@ -847,7 +943,7 @@ __global__ void __launch_bounds__(256) paged_add_weights_kernel(const PagedView 
 // how a call lays out its workspace; rows and dkm follow the kernel that takes it
 struct WsPlan {
     size_t desc, ml, o, lse2, scores, total;
-    int rows, dkm, slab_groups;
+    int wh, rows, dkm, slab_groups;
     long long score_stride;
 };
 static WsPlan plan_ws(int sm_count, bool f32_cache, const PagedView& c, const SeqView& s, size_t n_head, bool accumulate)
@@ -858,16 +954,17 @@ static WsPlan plan_ws(int sm_count, bool f32_cache, const PagedView& c, const Se
         p.rows = group == 1 ? 1 : group == 2 ? 2 : group <= 4 ? 4 : 8;
         p.dkm = c.dk <= 64 ? 64 : c.dk <= 128 ? 128 : 256;
     } else {
-        p.rows = group > 8 ? 16 : 8;
+        p.rows = group > 8 ? 16 : group > 4 ? 8 : 4;
         p.dkm = c.dk <= 64 ? 64 : c.dk <= 112 ? 112 : c.dk <= 128 ? 128 : c.dk <= 192 ? 192 : 256;
     }
     p.slab_groups = (group + p.rows - 1) / p.rows;
+    p.wh = p.rows == 16 ? 1 : c.heads % 4 == 0 ? 4 : c.heads % 2 == 0 ? 2 : 1;
     const size_t g = (size_t)sm_count * MAX_CTAS_PER_SM;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     p.desc = 0;
     p.ml = up(g * sizeof(int2));
-    p.o = p.ml + up(g * 2 * p.rows * 2 * sizeof(float));
-    p.lse2 = p.o + up(g * 2 * p.rows * p.dkm * sizeof(float));
+    p.o = p.ml + up(g * 2 * p.wh * p.rows * 2 * sizeof(float));
+    p.lse2 = p.o + up(g * 2 * p.wh * p.rows * p.dkm * sizeof(float));
     p.scores = p.lse2 + (accumulate ? up(s.n_seq * n_head * sizeof(float)) : 0);
     p.score_stride = (paged_capacity(c, s) + MAX_UNIT - 1) / MAX_UNIT * MAX_UNIT;
     p.total = p.scores + (accumulate ? s.n_seq * n_head * (size_t)p.score_stride * sizeof(float) : 0);
@@ -900,10 +997,13 @@ static nnb_status launch_workers(nnb_engine* e, void (*kern)(K...), size_t smem,
 template <int KS, typename TQ>
 static nnb_status launch_mma(nnb_engine* e, const PagedView& c, const SeqView& s, const DecodeArgs& a, const DecodeWs& ws, int* workers)
 {
-    static int one[64] = {}, two[64] = {};
-    if (ws.rows == 16)
-        return launch_workers(e, paged_decode_mma_kernel<KS, 2, TQ>, MmaCfg<KS, 2, sizeof(TQ) == 4>::SMEM, two, c, s, a, ws, workers);
-    return launch_workers(e, paged_decode_mma_kernel<KS, 1, TQ>, MmaCfg<KS, 1, sizeof(TQ) == 4>::SMEM, one, c, s, a, ws, workers);
+    constexpr bool PREC = sizeof(TQ) == 4;
+    static int n4[64] = {}, n8[64] = {}, n16[64] = {};
+    if (ws.rows == 16) return launch_workers(e, paged_decode_mma_kernel<KS, 16, TQ>, MmaCfg<KS, 16, PREC>::SMEM, n16, c, s, a, ws, workers);
+    if constexpr (PREC) {
+        if (ws.rows == 4) return launch_workers(e, paged_decode_mma_kernel<KS, 4, TQ>, MmaCfg<KS, 4, PREC>::SMEM, n4, c, s, a, ws, workers);
+    }
+    return launch_workers(e, paged_decode_mma_kernel<KS, 8, TQ>, MmaCfg<KS, 8, PREC>::SMEM, n8, c, s, a, ws, workers);
 }
 template <int FL, int NFI, int ROWS, typename TQ>
 static nnb_status launch_fma_rows(nnb_engine* e, const PagedView& c, const SeqView& s, const DecodeArgs& a, const DecodeWs& ws, int* workers)
@@ -927,7 +1027,7 @@ static nnb_status launch_decode(nnb_engine* e, bool f32_cache, const PagedView& 
 {
     const WsPlan p = plan_ws(e->sm_count, f32_cache, c, s, (size_t)a.n_head, accumulate);
     const DecodeWs ws{(int2*)(base + p.desc), (float*)(base + p.ml), (float*)(base + p.o), accumulate ? (float*)(base + p.lse2) : nullptr,
-                      accumulate ? (float*)(base + p.scores) : nullptr, p.score_stride, p.rows, p.dkm, p.slab_groups};
+                      accumulate ? (float*)(base + p.scores) : nullptr, p.score_stride, p.wh, p.rows, p.dkm, p.slab_groups};
     PdlOn pdl(e);
     int workers = 0;
     if (f32_cache) {
@@ -947,7 +1047,7 @@ static nnb_status launch_decode(nnb_engine* e, bool f32_cache, const PagedView& 
         }
     }
     const size_t smem = (size_t)(workers > 512 ? workers : 512) * sizeof(float);
-    NNB_CUDA(launch_ex(e, paged_join_kernel<TQ>, dim3((unsigned)workers, (unsigned)(a.group < p.rows ? a.group : p.rows)), dim3(128), smem, c, s, a, ws,
+    NNB_CUDA(launch_ex(e, paged_join_kernel<TQ>, dim3((unsigned)workers, (unsigned)(p.wh * p.rows)), dim3(128), smem, c, s, a, ws,
                        e->dev_flags));
     e->launches++;
     if (accumulate) {
