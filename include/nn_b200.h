@@ -380,7 +380,8 @@ nnb_status nnb_paged_evict(nnb_engine* e, const nnb_paged_cache* src, const nnb_
  *   if bit i % 32 of word i / 32 of d_allowed is 0:                         x = -inf.
  * Every pointer except d_logits / d_out may be NULL (that part is off; d_prompt_len NULL = 0).  r = d_repeat[s] <= 0 or 1 is
  * off.  Ids outside [0, vocab) are ignored (padding), lengths are clamped to [0, max_history].  Rows are the given strides
- * apart (elements, words; a stride of 0 for d_bias / d_allowed shares one row).  d_out may be d_logits with its stride. */
+ * apart (elements, words; a stride of 0 for d_bias / d_allowed shares one row).  d_out may be d_logits with its stride.
+ * vocab is at most 2^26. */
 typedef struct nnb_logits_config {
     const int32_t* d_history;
     size_t history_stride, max_history;

@@ -58,4 +58,13 @@ struct DeviceScope {
     }
 };
 
+// The operators' kernels are launched with the programmatic attribute: each waits for its predecessor itself, with pdl_wait
+// before its first access and in every thread, so that the chain of completions stays whole.
+struct PdlOn {
+    nnb_engine* e;
+    bool prev;
+    explicit PdlOn(nnb_engine* en) : e(en), prev(en->pdl) { e->pdl = true; }
+    ~PdlOn() { e->pdl = prev; }
+};
+
 }  // namespace nnb

@@ -23,14 +23,14 @@ __device__ __forceinline__ void store_one(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_one(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
 // ------------------------------------------------------------------------------------------------ division of the work
-// A CTA's four warps take wh KV heads at a time, wp = 4 / wh warps each: with four heads no warp has to wait for another.  An
+// A CTA's four warps take wh KV heads at a time, wp = 4 / wh warps each: fewer warps have to be joined at an item's end.  An
 // item is (sequence, wh KV heads, slab of query heads); its positions form units of 16 wp (8 wp for wide f32 rows), a tile for
 // each warp.  The work is cut evenly whatever the lengths: an item costs its units and ITEM_COST more for its beginning and
-// end, and worker w of G (one CTA each; G at most the whole cost U) takes what lies in [U w / G, U (w + 1) / G) of the batch
+// end (measured with 0 / 1 / 2 / 4: 86 / 73 / 67 / 67 us for 128 sequences of 0..640 positions), and worker w of G (one CTA each; G at most the whole cost U) takes what lies in [U w / G, U (w + 1) / G) of the batch
 // in order.  A worker finishes the items that lie inside its range; of an item that several workers share each leaves a
 // partial softmax (maximum, sum, weighted values) that paged_join_kernel folds in order.  A worker has at most two partial
 // items: slot 0 is one that began in an earlier worker, slot 1 one that begins here and goes on in the next.
-constexpr int MAX_CTAS_PER_SM = 4, MAX_UNIT = 64, ITEM_COST = 1;
+constexpr int MAX_CTAS_PER_SM = 4, MAX_UNIT = 64, ITEM_COST = 2;
 
 struct DecodeWs {
     int2* desc;      // (G): the split item that begins in worker w and its last worker; item -1: none
@@ -244,7 +244,7 @@ struct MmaCfg {
     static constexpr bool REGQ = KS * NSLAB * (THIRD ? 6 : 4) <= 64;        // query fragments in registers, else in shared memory
     static constexpr int QS = NSLAB * (THIRD ? 24 : 16), QROWS = REGQ ? 0 : QS;
     static constexpr int STAGE = 2 * TK * LD;                               // elements of a warp's key and value tile
-    static constexpr int NST = KS <= 8 && HEADS < 16 ? 3 : 2;
+    static constexpr int NST = KS <= 8 && HEADS < 16 ? 3 : 2;             // 3 CTAs of 2 stages instead of 2 of 3: 139 us for 96
     static constexpr int CTAS = KS == 4 ? (HEADS == 16 ? 2 : 4) : KS <= 8 ? 2 : 1;
     // a warp's result of an item is parked over the tile that it has just used: rows of PARK floats, then maximum and sum
     static constexpr int ROWS = 8 * NSLAB, PARK = DKM + (NSLAB == 1 ? 8 : 4);
@@ -958,7 +958,9 @@ static WsPlan plan_ws(int sm_count, bool f32_cache, const PagedView& c, const Se
         p.dkm = c.dk <= 64 ? 64 : c.dk <= 112 ? 112 : c.dk <= 128 ? 128 : c.dk <= 192 ? 192 : 256;
     }
     p.slab_groups = (group + p.rows - 1) / p.rows;
-    p.wh = p.rows == 16 ? 1 : c.heads % 4 == 0 ? 4 : c.heads % 2 == 0 ? 2 : 1;
+    // Measured with 1 / 2 / 4 heads: 128 sequences of 0..640 positions with 16 KV heads of 128 73.7 / 65.8 / 70.6 us, 32 of
+    // 256..2048 with 32 of 100 97.5 / 98.7 / 105 us, 64 of 1000..8192 with 8 of 128 206.6 / 206.8 / 210 us.
+    p.wh = p.rows == 16 || c.heads % 2 != 0 ? 1 : 2;
     const size_t g = (size_t)sm_count * MAX_CTAS_PER_SM;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     p.desc = 0;
@@ -970,14 +972,6 @@ static WsPlan plan_ws(int sm_count, bool f32_cache, const PagedView& c, const Se
     p.total = p.scores + (accumulate ? s.n_seq * n_head * (size_t)p.score_stride * sizeof(float) : 0);
     return p;
 }
-
-// launches with the programmatic attribute: the kernel waits for its predecessor itself (pdl_wait before its first access)
-struct PdlOn {
-    nnb_engine* e;
-    bool prev;
-    explicit PdlOn(nnb_engine* en) : e(en), prev(en->pdl) { e->pdl = true; }
-    ~PdlOn() { e->pdl = prev; }
-};
 
 template <typename... K>
 static nnb_status launch_workers(nnb_engine* e, void (*kern)(K...), size_t smem, int (&per_sm)[64], const PagedView& c, const SeqView& s, const DecodeArgs& a,
