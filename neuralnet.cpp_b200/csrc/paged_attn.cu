@@ -30,7 +30,8 @@ __device__ __forceinline__ void store_one(__nv_bfloat16* p, float x) { *p = __fl
 // in order.  A worker finishes the items that lie inside its range; of an item that several workers share each leaves a
 // partial softmax (maximum, sum, weighted values) that paged_join_kernel folds in order.  A worker has at most two partial
 // items: slot 0 is one that began in an earlier worker, slot 1 one that begins here and goes on in the next.
-constexpr int MAX_CTAS_PER_SM = 4, MAX_UNIT = 64, ITEM_COST = 2;
+constexpr int LONG_CALL = 96;  // units per worker from which on a call has a second set of workers
+constexpr int MAX_CTAS_PER_SM = 4, MAX_WORKERS = MAX_CTAS_PER_SM * 3 / 2 /* per SM, both sets */, MAX_UNIT = 64, ITEM_COST = 2;
 
 struct DecodeWs {
     int2* desc;      // (G): the split item that begins in worker w and its last worker; item -1: none
@@ -39,7 +40,7 @@ struct DecodeWs {
     float* lse2;     // (n_seq, n_head): log2 of the sum of exp, for the weights; or NULL
     float* scores;   // (n_seq, n_head, score_stride): scores in the log2 domain, for the weights; or NULL
     long long score_stride;
-    int wh;
+    int wh, wide;    // wide: workers of the first set
     int rows, dkm;   // query heads of an item per KV head, and the pitch of the partial results
     int slab_groups; // items per (sequence, wh KV heads): larger groups of query heads than a pass serves are cut
 };
@@ -66,9 +67,26 @@ __device__ __forceinline__ void next_item(UnitIter& it, const PagedView& c, cons
     } while (it.tiles == 0 && it.seq + 1 < s.n_seq);
 }
 
+// How the cost is dealt out.  The SMs of some GPCs get up to a fifth less of the memory's rate than others, so a long call's
+// last tenth goes to a second set of workers, half as many, which start wherever one of the first set ends (64 sequences of
+// 1000..8192 positions: 213 us without, 198 us with; with as many as the first set 200 us, with the last 15 % 203 us).
+struct Deal {
+    long long units, head;  // the whole, and what the first `wide` workers share evenly
+    int wide, rest;         // the other `rest` workers share what is left
+    __device__ __forceinline__ long long start(int w) const
+    {
+        return w <= wide ? head * w / wide : head + (units - head) * (w - wide) / rest;
+    }
+    // the worker that has position u: the last that starts at u or before
+    __device__ __forceinline__ int worker_of(long long u) const
+    {
+        return u < head ? (int)(((u + 1) * wide - 1) / head) : wide + (int)(((u - head + 1) * rest - 1) / (units - head));
+    }
+};
+
 // Called by all 128 threads: this worker's range of the cost and the place of its first unit; false if it has none.
-__device__ __forceinline__ bool find_work(const PagedView& c, const SeqView& s, int unit, int items_per_seq, UnitIter& it, long long& u0, long long& u1,
-                                          long long& units, int& workers, int* flags)
+__device__ __forceinline__ bool find_work(const PagedView& c, const SeqView& s, int unit, int items_per_seq, const DecodeWs& ws, UnitIter& it, long long& u0, long long& u1,
+                                          Deal& deal, int* flags)
 {
     __shared__ long long warp_sum[4], place;
     __shared__ int place_seq;
@@ -90,15 +108,17 @@ __device__ __forceinline__ bool find_work(const PagedView& c, const SeqView& s, 
     if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
     long long base = 0;
-    units = 0;
+    deal.units = 0;
     for (int i = 0; i < 4; ++i) {
         if (i < warp) base += warp_sum[i];
-        units += warp_sum[i];
+        deal.units += warp_sum[i];
     }
-    workers = (int)min((long long)gridDim.x, units);
-    if ((int)blockIdx.x >= workers) return false;
-    u0 = units * blockIdx.x / workers;
-    u1 = units * (blockIdx.x + 1) / workers;
+    deal.wide = (int)min((long long)ws.wide, deal.units);
+    deal.rest = deal.units >= (long long)LONG_CALL * ws.wide ? gridDim.x - ws.wide : 0;
+    deal.head = deal.rest ? deal.units * 9 / 10 : deal.units;
+    if ((int)blockIdx.x >= deal.wide + deal.rest) return false;
+    u0 = deal.start(blockIdx.x);
+    u1 = deal.start(blockIdx.x + 1);
     base += incl - mine;
     if (u0 >= base && u0 < base + mine) {
         int i = first;
@@ -123,9 +143,6 @@ __device__ __forceinline__ bool find_work(const PagedView& c, const SeqView& s, 
     }
     return true;
 }
-// the worker that has position u of the cost: the largest w with floor(units w / G) <= u
-__device__ __forceinline__ int worker_of(long long u, long long units, int g) { return (int)(((u + 1) * g - 1) / units); }
-
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void* p)
 {
     const uint32_t a = (uint32_t)__cvta_generic_to_shared(p);
@@ -141,6 +158,33 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the same with nothing to add to
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// two f32 operations in one instruction
+__device__ __forceinline__ unsigned long long two(float x, float y)
+{
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b)
+{
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(two(x, y)), "l"(two(a, b)));
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(r));
+}
+// (x, y) += (a, b) * (p, q)
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float p, float q)
+{
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(two(a, b)), "l"(two(p, q)), "l"(two(x, y)));
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(x), "=f"(y) : "l"(r));
 }
 __device__ __forceinline__ uint32_t pack_rn(float lo, float hi)
 {
@@ -270,9 +314,9 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
     pdl_launch();
     const int wp = 4 / ws.wh, unit = TK * wp, in_head = warp / wp, items_per_seq = c.heads / ws.wh * ws.slab_groups;
     UnitIter ct;
-    long long u_begin, u_end, units;
-    int workers;
-    const bool work = find_work(c, s, unit, items_per_seq, ct, u_begin, u_end, units, workers, flags);
+    long long u_begin, u_end;
+    Deal deal;
+    const bool work = find_work(c, s, unit, items_per_seq, ws, ct, u_begin, u_end, deal, flags);
     if (tid == 0) ws.desc[blockIdx.x] = make_int2(-1, -1);
     if (!work) return;
     // cost left for the computing and for the issuing side, which runs NST units ahead
@@ -283,6 +327,7 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
     const unsigned row_bytes = (unsigned)c.pitch * 2;
     const int my_row = lane / CHP, my_ch = lane % CHP;
     const bool my_live = my_ch < c.pitch / 8;
+    const unsigned my_off = my_row * row_bytes + min(my_ch, c.pitch / 8 - 1) * 16;
     // Pages of a multiple of 16 positions: a tile lies in one page and its rows follow one another.  Otherwise each lane
     // looks up the row of one position of the tile.
     const bool whole_tiles = c.page % TK == 0;
@@ -295,48 +340,53 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
     int ahead = it.n - it.tile * unit - my_pos;  // positions of the item from this lane's on
     unsigned long long exist = 0;  // which of the 16 positions of each tile under way exist (a bit each, the oldest tile lowest)
     if (ahead > 0) page_id = table_row[col];
-    auto issue = [&](int stage, int age) {
-        if (to_issue > 0) {
-            unsigned mask = 0;
-            int row = -1;
-            if (ahead > 0) {
-                if ((unsigned)page_id < (unsigned)c.n_pages)
-                    row = (page_id * c.heads + head) * c.page + slot_in_page;
-                else
-                    paged_flag(flags, PAGED_BAD_PAGE);
-            }
-            __nv_bfloat16* kt = ring + stage * C::STAGE + my_row * LD + my_ch * 8;
-            __nv_bfloat16* vt = kt + TK * LD;
-            if (whole_tiles) {
-                const int n = row >= 0 ? min(ahead, TK) : 0;
-                mask = (1u << n) - 1u;
-                const size_t off = n ? (size_t)(unsigned)row * row_bytes + my_row * row_bytes + my_ch * 16 : 0;
-                const char* kp = kbase + off;
-                const char* vp = vbase + off;
-                const int lim = my_live ? n - my_row : 0;  // row i * RPI + my_row exists: i * RPI < lim
-                if (CH == CHP || my_ch < CH)
-#pragma unroll
-                    for (int i = 0; i < TK / RPI; ++i) {
-                        const bool ok = i * RPI < lim;
-                        cp16_zfill(kt + i * RPI * LD, ok ? kp : kbase, ok);
-                        cp16_zfill(vt + i * RPI * LD, ok ? vp : vbase, ok);
-                        kp += RPI * row_bytes;
-                        vp += RPI * row_bytes;
-                    }
-            } else {
-                mask = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+    // The tile's keys are requested as soon as the scores of the one before in this stage are formed, its values (and the
+    // commit) after that one's products.
+    const char* next_kp = kbase;  // whole tiles: this lane's first chunk; otherwise the row of its position is in next_row
+    int next_row = -1, next_lim = 0;
+    auto issue_tile = [&](__nv_bfloat16* dst, const char* base, const char* first) {
+        if (whole_tiles) {
+            if (CH == CHP || my_ch < CH)
 #pragma unroll
                 for (int i = 0; i < TK / RPI; ++i) {
-                    const int src = __shfl_sync(0xffffffffu, row, i * RPI + my_row);
-                    const bool ok = src >= 0 && my_live;
-                    const size_t off = ok ? (size_t)(unsigned)src * row_bytes + my_ch * 16 : 0;
-                    if (CH == CHP || my_ch < CH) {
-                        cp16_zfill(kt + i * RPI * LD, kbase + off, ok);
-                        cp16_zfill(vt + i * RPI * LD, vbase + off, ok);
-                    }
+                    cp16_zfill(dst + i * RPI * LD, first, i * RPI < next_lim);
+                    first += RPI * row_bytes;
                 }
+        } else {
+#pragma unroll
+            for (int i = 0; i < TK / RPI; ++i) {
+                const int src = __shfl_sync(0xffffffffu, next_row, i * RPI + my_row);
+                const bool ok = src >= 0 && my_live;
+                if (CH == CHP || my_ch < CH) cp16_zfill(dst + i * RPI * LD, base + (ok ? (size_t)(unsigned)src * row_bytes + my_ch * 16 : 0), ok);
             }
-            exist |= (unsigned long long)mask << (16 * age);
+        }
+    };
+    auto issue_keys = [&](int stage, int age) {
+        if (to_issue <= 0) return;
+        unsigned mask = 0;
+        int row = -1;
+        if (ahead > 0) {
+            if ((unsigned)page_id < (unsigned)c.n_pages)
+                row = (page_id * c.heads + head) * c.page + slot_in_page;
+            else
+                paged_flag(flags, PAGED_BAD_PAGE);
+        }
+        if (whole_tiles) {
+            const int n = row >= 0 ? min(ahead, TK) : 0;
+            mask = (1u << n) - 1u;
+            // (all 16 rows lie in the page, or in the pool's first for a tile without any: every address is in the pool)
+            next_kp = kbase + ((size_t)(unsigned)(n ? row : 0) * row_bytes + my_off);
+            next_lim = my_live ? n - my_row : 0;  // row i * RPI + my_row exists: i * RPI < next_lim
+        } else {
+            mask = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+            next_row = row;
+        }
+        issue_tile(ring + stage * C::STAGE + my_row * LD + my_ch * 8, kbase, next_kp);
+        exist |= (unsigned long long)mask << (16 * age);
+    };
+    auto issue_values = [&](int stage) {
+        if (to_issue > 0) {
+            issue_tile(ring + stage * C::STAGE + (TK + my_row) * LD + my_ch * 8, vbase, next_kp + (vbase - kbase));
             --to_issue;
             if (++it.tile == it.tiles) to_issue -= ITEM_COST;
             if (to_issue > 0) {
@@ -363,12 +413,15 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
         asm volatile("cp.async.commit_group;\n" ::);
     };
 #pragma unroll
-    for (int i = 0; i < NST; ++i) issue(i, i);
+    for (int i = 0; i < NST; ++i) {
+        issue_keys(i, i);
+        issue_values(i);
+    }
 
     const float scale2 = a.scale * 1.44269504088896341f;
     uint32_t qa[C::REGQ ? NSLAB : 1][C::REGQ ? KS : 1][4], qb[C::REGQ && C::THIRD ? NSLAB : 1][C::REGQ && C::THIRD ? KS : 1][2];
-    // o[..][0..1]: row g, o[..][2..3]: row g + 8.  With f32 outputs row g (the leading pieces) is added in f32 after every tile:
-    // tensor cores truncate their sums, which only the small pieces can afford over a long context.
+    // o[..][0..1]: row g, o[..][2..3]: row g + 8.  With f32 outputs they are added in f32 after every tile: tensor cores truncate
+    // their sums, which f32 results cannot afford over a long context.
     float o[NSLAB][NT][4], m[NSLAB], l[NSLAB];
     bool fresh = true, starts_here = false;
     int stage = 0;
@@ -456,8 +509,10 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         float(&d)[4] = acc[sl][j][ks & 1];
-                        if (ks < 2) d[0] = d[1] = d[2] = d[3] = 0.0f;
-                        mma16816(d, f[0], f[1], f[2], f[3], b[2 * j], b[2 * j + 1]);
+                        if (ks < 2)
+                            mma16816_first(d, f[0], f[1], f[2], f[3], b[2 * j], b[2 * j + 1]);
+                        else
+                            mma16816(d, f[0], f[1], f[2], f[3], b[2 * j], b[2 * j + 1]);
                         if constexpr (C::THIRD) mma16816(d, f2[0], 0u, f2[1], 0u, b[2 * j], b[2 * j + 1]);
                     }
                 }
@@ -482,6 +537,11 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
                         for (int i = 0; i < 2; ++i)
                             if (!((live >> (8 * j + 2 * t4 + i)) & 1u)) x[sl][j][i] = -INFINITY;
         }
+        const bool ends = ct.tile + 1 == ct.tiles;
+        left -= ends ? 1 + ITEM_COST : 1;
+        const bool last = left <= 0, closing = ends || last;  // a closing tile's stage is needed once more
+        __syncwarp();
+        if (!closing) issue_keys(stage, NST - 1);
         float corr[NSLAB];
         bool moved = false;
 #pragma unroll
@@ -545,26 +605,21 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
                 for (int j = 0; j < 2; ++j) {
                     float(&d)[4] = o[sl][2 * np + j];
                     if constexpr (PREC) {
-                        float y[4] = {0.0f, 0.0f, d[2], d[3]};
-                        mma16816(y, pa[sl][0], pa[sl][1], pa[sl][2], pa[sl][3], b[2 * j], b[2 * j + 1]);
+                        float y[4];
+                        mma16816_first(y, pa[sl][0], pa[sl][1], pa[sl][2], pa[sl][3], b[2 * j], b[2 * j + 1]);
                         if constexpr (C::THIRD) mma16816(y, pb[sl][0], 0u, pb[sl][1], 0u, b[2 * j], b[2 * j + 1]);
-                        d[0] = __fadd_rn(d[0], y[0]);
-                        d[1] = __fadd_rn(d[1], y[1]);
-                        d[2] = y[2];
-                        d[3] = y[3];
+                        add2(d[0], d[1], y[0], y[1]);
+                        add2(d[2], d[3], y[2], y[3]);
                     } else {
                         mma16816(d, pa[sl][0], pa[sl][1], pa[sl][2], pa[sl][3], b[2 * j], b[2 * j + 1]);
                     }
                 }
         }
         __syncwarp();
-        const bool ends = ct.tile + 1 == ct.tiles;
-        left -= ends ? 1 + ITEM_COST : 1;
-        const bool last = left <= 0;
-        if (ends || last) {  // fold the four warps' results
+        if (closing) {  // fold the four warps' results
             const bool whole = starts_here && ends;
             if (tid == 0 && starts_here && !ends)
-                ws.desc[blockIdx.x] = make_int2(ct.seq * items_per_seq + ct.hs, worker_of(u_end - 1 + (ct.tiles - 1 - ct.tile), units, workers));
+                ws.desc[blockIdx.x] = make_int2(ct.seq * items_per_seq + ct.hs, deal.worker_of(u_end - 1 + (ct.tiles - 1 - ct.tile)));
             float* park = reinterpret_cast<float*>(ring + stage * C::STAGE);
 #pragma unroll
             for (int sl = 0; sl < NSLAB; ++sl) {
@@ -591,7 +646,8 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
             fresh = true;
         }
         if (last) break;
-        issue(stage, NST - 1);
+        if (closing) issue_keys(stage, NST - 1);
+        issue_values(stage);
         stage = stage + 1 == NST ? 0 : stage + 1;
         if (++ct.tile == ct.tiles) next_item(ct, c, s, unit, items_per_seq, flags);
     }
@@ -628,9 +684,9 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
     float* qs = smem_f + (size_t)4 * NST * stage_len + (size_t)in_head * ROWS * ld;  // one copy per KV head of the CTA
     float* ps = smem_f + (size_t)4 * NST * stage_len + (size_t)ws.wh * ROWS * ld + warp * TK * ROWS;  // this warp's probabilities, (position, row)
     UnitIter ct;
-    long long u_begin, u_end, units;
-    int workers;
-    const bool work = find_work(c, s, unit, items_per_seq, ct, u_begin, u_end, units, workers, flags);
+    long long u_begin, u_end;
+    Deal deal;
+    const bool work = find_work(c, s, unit, items_per_seq, ws, ct, u_begin, u_end, deal, flags);
     if (tid == 0) ws.desc[blockIdx.x] = make_int2(-1, -1);
     if (!work) return;
     long long left = u_end - u_begin, to_issue = left;
@@ -735,19 +791,24 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
         const unsigned live = (unsigned)exist & 0xffffu;
         exist >>= 16;
         // scores: LPK lanes per position, every LPK-th vector of the row each
-        float x[ROWS];
+        float x[ROWS], x_odd[ROWS];
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) x[r] = 0.0f;
+        for (int r = 0; r < ROWS; ++r) x[r] = x_odd[r] = 0.0f;
+#pragma unroll 4
         for (int ch = sub; ch < chunks; ch += LPK) {
             const float4 kf = *reinterpret_cast<const float4*>(kt + key * ld + ch * 4);
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 const float4 qf = *reinterpret_cast<const float4*>(qs + r * ld + ch * 4);
-                x[r] = fmaf(qf.x, kf.x, fmaf(qf.y, kf.y, fmaf(qf.z, kf.z, fmaf(qf.w, kf.w, x[r]))));
+                fma2(x[r], x_odd[r], qf.x, qf.y, kf.x, kf.y);
+                fma2(x[r], x_odd[r], qf.z, qf.w, kf.z, kf.w);
             }
         }
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) x[r] += x_odd[r];
         const bool on = (live >> key) & 1u;
         float corr[ROWS];
+        bool moved = false;  // the same for the whole warp
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
 #pragma unroll
@@ -760,13 +821,15 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
             for (int d = LPK; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             top = fmaxf(top, m[r]);
             const float base = top == -INFINITY ? 0.0f : top;
-            corr[r] = exp2f(m[r] - base);
+            corr[r] = exp2_fast(m[r] - base);
+            moved |= top != m[r];
             m[r] = top;
-            x[r] = exp2f(x[r] - base);
+            x[r] = exp2_fast(x[r] - base);
             l[r] = fmaf(l[r], corr[r], x[r]);  // the LPK lanes of a position hold the same share: divided out at the end
             if (sub == 0) ps[key * ROWS + r] = x[r];
         }
         __syncwarp();
+        if (moved)
 #pragma unroll
         for (int r = 0; r < ROWS; ++r)
 #pragma unroll
@@ -787,10 +850,8 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
 #pragma unroll
                     for (int r = 0; r < ROWS; ++r) {
                         const float p = ps[t * ROWS + r];
-                        o[r][j].x = fmaf(p, vf.x, o[r][j].x);
-                        o[r][j].y = fmaf(p, vf.y, o[r][j].y);
-                        o[r][j].z = fmaf(p, vf.z, o[r][j].z);
-                        o[r][j].w = fmaf(p, vf.w, o[r][j].w);
+                        fma2(o[r][j].x, o[r][j].y, p, p, vf.x, vf.y);
+                        fma2(o[r][j].z, o[r][j].w, p, p, vf.z, vf.w);
                     }
                 }
             }
@@ -802,7 +863,7 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
         if (ends || last) {  // fold the lanes' and the warps' results
             const bool whole = starts_here && ends;
             if (tid == 0 && starts_here && !ends)
-                ws.desc[blockIdx.x] = make_int2(ct.seq * items_per_seq + ct.hs, worker_of(u_end - 1 + (ct.tiles - 1 - ct.tile), units, workers));
+                ws.desc[blockIdx.x] = make_int2(ct.seq * items_per_seq + ct.hs, deal.worker_of(u_end - 1 + (ct.tiles - 1 - ct.tile)));
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 l[r] = warp_sum(l[r]) * (1.0f / LPK);
@@ -961,7 +1022,7 @@ static WsPlan plan_ws(int sm_count, bool f32_cache, const PagedView& c, const Se
     // Measured with 1 / 2 / 4 heads: 128 sequences of 0..640 positions with 16 KV heads of 128 73.7 / 65.8 / 70.6 us, 32 of
     // 256..2048 with 32 of 100 97.5 / 98.7 / 105 us, 64 of 1000..8192 with 8 of 128 206.6 / 206.8 / 210 us.
     p.wh = p.rows == 16 || c.heads % 2 != 0 ? 1 : 2;
-    const size_t g = (size_t)sm_count * MAX_CTAS_PER_SM;
+    const size_t g = (size_t)sm_count * MAX_WORKERS;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     p.desc = 0;
     p.ml = up(g * sizeof(int2));
@@ -975,7 +1036,7 @@ static WsPlan plan_ws(int sm_count, bool f32_cache, const PagedView& c, const Se
 
 template <typename... K>
 static nnb_status launch_workers(nnb_engine* e, void (*kern)(K...), size_t smem, int (&per_sm)[64], const PagedView& c, const SeqView& s, const DecodeArgs& a,
-                                 const DecodeWs& ws, int* workers)
+                                 DecodeWs ws, int* workers)
 {
     int& n = per_sm[e->device & 63];  // resident CTAs per SM, by device
     if (n == 0) {
@@ -983,7 +1044,10 @@ static nnb_status launch_workers(nnb_engine* e, void (*kern)(K...), size_t smem,
         NNB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, 128, smem));
         n = n < 1 ? 1 : n > MAX_CTAS_PER_SM ? MAX_CTAS_PER_SM : n;
     }
-    *workers = e->sm_count * n;
+    ws.wide = e->sm_count * n;
+    // (the lengths are on the device: the table's capacity bounds the cost from above)
+    const size_t unit = 16 * (4 / ws.wh), most = (size_t)s.n_seq * (c.heads / ws.wh) * ws.slab_groups * (ceil_div((size_t)paged_capacity(c, s), unit) + ITEM_COST);
+    *workers = most >= (size_t)LONG_CALL * ws.wide ? ws.wide + ws.wide / 2 : ws.wide;
     NNB_CUDA(launch_ex(e, kern, dim3((unsigned)*workers), dim3(128), smem, c, s, a, ws, e->dev_flags));
     e->launches++;
     return NNB_OK;
@@ -1020,8 +1084,8 @@ template <typename TQ>
 static nnb_status launch_decode(nnb_engine* e, bool f32_cache, const PagedView& c, const SeqView& s, const DecodeArgs& a, bool accumulate, char* base)
 {
     const WsPlan p = plan_ws(e->sm_count, f32_cache, c, s, (size_t)a.n_head, accumulate);
-    const DecodeWs ws{(int2*)(base + p.desc), (float*)(base + p.ml), (float*)(base + p.o), accumulate ? (float*)(base + p.lse2) : nullptr,
-                      accumulate ? (float*)(base + p.scores) : nullptr, p.score_stride, p.wh, p.rows, p.dkm, p.slab_groups};
+    DecodeWs ws{(int2*)(base + p.desc), (float*)(base + p.ml), (float*)(base + p.o), accumulate ? (float*)(base + p.lse2) : nullptr,
+                      accumulate ? (float*)(base + p.scores) : nullptr, p.score_stride, p.wh, 0, p.rows, p.dkm, p.slab_groups};
     PdlOn pdl(e);
     int workers = 0;
     if (f32_cache) {
