@@ -276,7 +276,10 @@ static nnb_status launch_append(nnb_engine* e, const PagedView& c, const SeqView
     void (*kern)(PagedView, SeqView, AppendArgs, int, int*);
     if (staged) {
         kern = vec == 8 ? paged_append_kernel<TI, TC, 8, true> : vec == 2 ? paged_append_kernel<TI, TC, 2, true> : paged_append_kernel<TI, TC, 1, true>;
-        NNB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)APPEND_SMEM));
+        static bool raised[64][3] = {};  // the attribute is per device
+        bool& done = raised[e->device & 63][vec == 8 ? 0 : vec == 2 ? 1 : 2];
+        if (!done) NNB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)APPEND_SMEM));
+        done = true;
     } else {
         kern = vec == 8 ? paged_append_kernel<TI, TC, 8, false> : vec == 2 ? paged_append_kernel<TI, TC, 2, false> : paged_append_kernel<TI, TC, 1, false>;
     }
@@ -544,7 +547,7 @@ nnb_status nnb_paged_append(nnb_engine* e, const nnb_paged_cache* c, const nnb_p
     NNB_TRY(paged_check_seqs(who, c, s, &sv));
     NNB_REQUIRE(t, "%s: tokens are NULL", who);
     NNB_REQUIRE(t->dtype == NNB_F32 || t->dtype == NNB_BF16, "%s: dtype %d is neither f32 nor bf16", who, t->dtype);
-    NNB_REQUIRE(t->n_rows <= (size_t)INT32_MAX, "%s: more than 2^31 - 1 tokens", who);
+    NNB_REQUIRE(t->n_rows <= (1u << 30), "%s: more than 2^30 tokens", who);
     NNB_REQUIRE(t->d_row_start || t->n_rows == (size_t)s->n_seq, "%s: %zu tokens for %d sequences need d_row_start", who, t->n_rows, s->n_seq);
     const size_t kv_row = (size_t)c->n_head_kv * c->dk, q_row = t->n_head > 0 ? (size_t)t->n_head * c->dk : 0;
     NNB_REQUIRE(t->n_rows == 0 || (t->d_k && t->d_v), "%s: keys or values are NULL", who);

@@ -23,20 +23,21 @@ __device__ __forceinline__ void store_one(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store_one(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
 // ------------------------------------------------------------------------------------------------ division of the work
-// A CTA's four warps take wh KV heads at a time, wp = 4 / wh warps each: fewer warps have to be joined at an item's end.  An
-// item is (sequence, wh KV heads, slab of query heads); its positions form units of 16 wp (8 wp for wide f32 rows), a tile for
-// each warp.  The work is cut evenly whatever the lengths: an item costs its units and ITEM_COST more for its beginning and
-// end (measured with 0 / 1 / 2 / 4: 86 / 73 / 67 / 67 us for 128 sequences of 0..640 positions), and worker w of G (one CTA each; G at most the whole cost U) takes what lies in [U w / G, U (w + 1) / G) of the batch
-// in order.  A worker finishes the items that lie inside its range; of an item that several workers share each leaves a
-// partial softmax (maximum, sum, weighted values) that paged_join_kernel folds in order.  A worker has at most two partial
-// items: slot 0 is one that began in an earlier worker, slot 1 one that begins here and goes on in the next.
+// A CTA's four warps take wh (1 or 2) KV heads at a time, wp = 4 / wh warps each: with two, fewer warps have to be joined at
+// an item's end.  An item is (sequence, wh KV heads, slab of query heads); its positions form units of 16 wp (8 wp for wide
+// f32 rows), a tile for each warp.  The work is cut evenly whatever the lengths: an item costs its units and ITEM_COST more
+// for its beginning and end (measured with 0 / 1 / 2 / 4: 86 / 73 / 67 / 67 us for 128 sequences of 0..640 positions), and
+// each worker (one CTA; at most as many as the whole cost) takes an even share of the batch in order.  A worker finishes the
+// items that lie inside its range; of an item that several workers share each leaves a partial softmax (maximum, sum,
+// weighted values) that paged_join_kernel folds in order.  A worker has at most two partial items: slot 0 is one that began
+// in an earlier worker, slot 1 one that begins here and goes on in the next.
 constexpr int LONG_CALL = 96;  // units per worker from which on a call has a second set of workers
 constexpr int MAX_CTAS_PER_SM = 4, MAX_WORKERS = MAX_CTAS_PER_SM * 3 / 2 /* per SM, both sets */, MAX_UNIT = 64, ITEM_COST = 2;
 
 struct DecodeWs {
-    int2* desc;      // (G): the split item that begins in worker w and its last worker; item -1: none
-    float* ml;       // (G, 2, wh, rows, 2): maximum (log2 domain) and sum of a partial softmax
-    float* o;        // (G, 2, wh, rows, dkm): its weighted values
+    int2* desc;      // (workers): the split item that begins in a worker and its last worker; item -1: none
+    float* ml;       // (workers, 2, wh, rows, 2): maximum (log2 domain) and sum of a partial softmax
+    float* o;        // (workers, 2, wh, rows, dkm): its weighted values
     float* lse2;     // (n_seq, n_head): log2 of the sum of exp, for the weights; or NULL
     float* scores;   // (n_seq, n_head, score_stride): scores in the log2 domain, for the weights; or NULL
     long long score_stride;
@@ -89,12 +90,13 @@ __device__ __forceinline__ bool find_work(const PagedView& c, const SeqView& s, 
                                           Deal& deal, int* flags)
 {
     __shared__ long long warp_sum[4], place;
-    __shared__ int place_seq;
+    __shared__ int place_seq, place_n;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (s.n_seq + 127) / 128, first = min(s.n_seq, tid * per), last = min(s.n_seq, first + per);
+    int n_seen = 0;  // the length that was read last: the only one where each thread has one sequence
     auto cost = [&](int i) {
-        const int n = paged_len(c, s, i, flags);
-        return n ? (n + unit - 1) / unit + ITEM_COST : 0;
+        n_seen = paged_len(c, s, i, flags);
+        return n_seen ? (n_seen + unit - 1) / unit + ITEM_COST : 0;
     };
     long long mine = 0;
     for (int i = first; i < last; ++i) mine += cost(i);
@@ -123,17 +125,20 @@ __device__ __forceinline__ bool find_work(const PagedView& c, const SeqView& s, 
     if (u0 >= base && u0 < base + mine) {
         int i = first;
         long long left = u0 - base;
-        for (; i + 1 < last; ++i) {
-            const long long n = (long long)cost(i) * items_per_seq;
-            if (left < n) break;
-            left -= n;
-        }
+        if (per > 1)
+            for (;; ++i) {
+                const long long n = (long long)cost(i) * items_per_seq;
+                if (left < n || i + 1 == last) break;
+                left -= n;
+            }
         place_seq = i;
+        place_n = n_seen;
         place = left;
     }
     __syncthreads();
     it.seq = place_seq;
-    load_seq(it, c, s, unit, flags);
+    it.n = place_n;
+    it.tiles = (it.n + unit - 1) / unit;
     it.hs = (int)(place / (it.tiles + ITEM_COST));
     it.tile = (int)(place % (it.tiles + ITEM_COST));
     if (it.tile >= it.tiles) {  // the range begins in what the end of an item costs
@@ -222,15 +227,6 @@ __device__ __forceinline__ void prefetch_queries(const PagedView& c, const Decod
     for (int b = (threadIdx.x & 31) * 128; b < bytes; b += 32 * 128) asm volatile("prefetch.global.L1 [%0];\n" ::"l"((const char*)q + b));
 }
 
-// the warps of a KV head (all of the CTA's where a head has more than one: they are at the same unit)
-__device__ __forceinline__ void sync_head(int wp)
-{
-    if (wp == 1)
-        __syncwarp();
-    else
-        __syncthreads();
-}
-
 // Folds the results that the wp warps of a KV head have parked (rows of STRIDE floats, then maximum and sum per row; warps
 // warp_stride floats apart) and writes them: outputs if the item is whole, a partial result otherwise.
 template <int DKM, int STRIDE, int ROWS, typename TQ>
@@ -293,7 +289,7 @@ struct MmaCfg {
     // a warp's result of an item is parked over the tile that it has just used: rows of PARK floats, then maximum and sum
     static constexpr int ROWS = 8 * NSLAB, PARK = DKM + (NSLAB == 1 ? 8 : 4);
     static_assert((ROWS * PARK + 2 * ROWS) * 4 <= STAGE * 2, "a parked result fits in a stage");
-    static constexpr size_t SMEM = (size_t)4 * NST * STAGE * 2 + (size_t)(HEADS == 16 ? 1 : 4) * QROWS * LD * 2;  // queries: a copy per KV head of the CTA
+    static constexpr size_t SMEM = (size_t)4 * NST * STAGE * 2 + (size_t)(HEADS == 16 ? 1 : 2) * QROWS * LD * 2;  // queries: for each KV head of the CTA
 };
 
 template <int KS, int HEADS, typename TQ>
@@ -336,6 +332,7 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
     UnitIter it = ct;
     int col = (it.tile * unit + my_pos) / c.page, slot_in_page = (it.tile * unit + my_pos) % c.page, page_id = -1;
     int head = it.hs / ws.slab_groups * ws.wh + in_head;
+    if (warp % wp == 0) prefetch_queries<TQ>(c, a, ws, it.seq, head, it.hs % ws.slab_groups * ws.rows);
     const int32_t* table_row = s.table + (long long)it.seq * s.stride;
     int ahead = it.n - it.tile * unit - my_pos;  // positions of the item from this lane's on
     unsigned long long exist = 0;  // which of the 16 positions of each tile under way exist (a bit each, the oldest tile lowest)
@@ -431,7 +428,7 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
         if (fresh) {  // a new item: its queries
             fresh = false;
             starts_here = ct.tile == 0;
-            if (!C::REGQ) sync_head(wp);
+            if (!C::REGQ) __syncthreads();
 #pragma unroll
             for (int sl = 0; sl < NSLAB; ++sl) {
                 m[sl] = -INFINITY;
@@ -472,7 +469,7 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
                     }
                 }
             }
-            if (!C::REGQ) sync_head(wp);
+            if (!C::REGQ) __syncthreads();
         }
         asm volatile("cp.async.wait_group %0;\n" ::"n"(NST - 1) : "memory");
         __syncwarp();
@@ -639,10 +636,10 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
                 for (int i = 0; i < NT; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[sl][i][0], o[sl][i][1]);
                 if (t4 == 0) *reinterpret_cast<float2*>(park + C::ROWS * C::PARK + (sl * 8 + g) * 2) = make_float2(m[sl], ls);
             }
-            sync_head(wp);
+            __syncthreads();
             fold_warps<C::DKM, C::PARK, C::ROWS, TQ>(reinterpret_cast<const float*>(smem_raw) + (in_head * wp * NST + stage) * (C::STAGE / 2),
                                                      NST * (C::STAGE / 2), wp, c, a, ws, ct.seq, hk, row0, whole, starts_here ? 1 : 0);
-            sync_head(wp);
+            __syncthreads();
             fresh = true;
         }
         if (last) break;
@@ -665,7 +662,7 @@ struct FmaCfg {
     static __host__ __device__ constexpr int ld(int pitch) { return pitch + (4 * LPK + 32 - pitch % 32) % 32; }
     static __host__ __device__ constexpr size_t smem(int pitch)
     {
-        return ((size_t)4 * NST * 2 * TK * ld(pitch) + (size_t)4 * ROWS * ld(pitch) + 4 * TK * ROWS) * sizeof(float);
+        return ((size_t)4 * NST * 2 * TK * ld(pitch) + (size_t)2 * ROWS * ld(pitch) + 4 * TK * ROWS) * sizeof(float);
     }
 };
 
@@ -699,6 +696,7 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
     UnitIter it = ct;
     int col = (it.tile * unit + my_pos) / c.page, slot_in_page = (it.tile * unit + my_pos) % c.page, page_id = -1;
     int head = it.hs / ws.slab_groups * ws.wh + in_head;
+    if (warp % wp == 0) prefetch_queries<TQ>(c, a, ws, it.seq, head, it.hs % ws.slab_groups * ws.rows);
     const int32_t* table_row = s.table + (long long)it.seq * s.stride;
     int ahead = it.n - it.tile * unit - my_pos;
     unsigned long long exist = 0;
@@ -769,12 +767,12 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
             fresh = false;
             starts_here = ct.tile == 0;
             const TQ* q = (const TQ*)a.q + (long long)ct.seq * a.q_stride + (long long)(hk * a.group + row0) * c.dk;
-            sync_head(wp);
+            __syncthreads();
 #pragma unroll
             for (int r = 0; r < ROWS; ++r)
                 for (int f = tid & (32 * wp - 1); f < c.pitch; f += 32 * wp)
                     qs[r * ld + f] = row0 + r < a.group && f < c.dk ? load_one(q + r * c.dk + f) : 0.0f;
-            sync_head(wp);
+            __syncthreads();
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 m[r] = -INFINITY;
@@ -831,14 +829,14 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
         __syncwarp();
         if (moved)
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r)
+            for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-            for (int j = 0; j < NFI; ++j) {
-                o[r][j].x *= corr[r];
-                o[r][j].y *= corr[r];
-                o[r][j].z *= corr[r];
-                o[r][j].w *= corr[r];
-            }
+                for (int j = 0; j < NFI; ++j) {
+                    o[r][j].x *= corr[r];
+                    o[r][j].y *= corr[r];
+                    o[r][j].z *= corr[r];
+                    o[r][j].w *= corr[r];
+                }
 #pragma unroll
         for (int i = 0; i < TK / RPI; ++i) {
             const int t = i * RPI + lane / FL;
@@ -888,10 +886,10 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
                     park[ROWS * C::DKM + 2 * r + 1] = l[r];
                 }
             }
-            sync_head(wp);
+            __syncthreads();
             fold_warps<C::DKM, C::DKM, ROWS, TQ>(smem_f + (in_head * wp * NST + stage) * stage_len, NST * stage_len, wp, c, a, ws, ct.seq, hk, row0, whole,
                                                  starts_here ? 1 : 0);
-            sync_head(wp);
+            __syncthreads();
             fresh = true;
         }
         if (last) break;

@@ -81,7 +81,8 @@ def _call(eng, fn, *args):
     if ptr == torch._C._cuda_getCurrentRawStream(eng.device.index):
         check(fn(eng._h, *args))
         return
-    cur, own = torch.cuda.current_stream(eng.device), torch.cuda.ExternalStream(ptr, device=eng.device)
+    cur = torch.cuda.current_stream(eng.device)
+    own = torch.cuda.ExternalStream(ptr, device=eng.device) if ptr else torch.cuda.default_stream(eng.device)
     own.wait_stream(cur)
     try:
         check(fn(eng._h, *args))

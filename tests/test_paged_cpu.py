@@ -51,7 +51,8 @@ def test_pitch_and_row(pkg):
 
 BAD_CACHE = [(dict(d_k=None), "no keys"), (dict(d_v=None), "no keys"), (dict(dtype=2), "dtype"), (dict(n_pages=0), "no pages"),
              (dict(page_size=0), "no pages"), (dict(n_head_kv=0), "no pages"), (dict(n_head_kv=-1), "no pages"), (dict(dk=0), "head size"),
-             (dict(dk=65), "head size"), (dict(dk=258), "head size"), (dict(d_k=FAKE + 8), "16-byte"), (dict(d_v=FAKE + 2), "16-byte")]
+             (dict(dk=65), "head size"), (dict(dk=258), "head size"), (dict(d_k=FAKE + 8), "16-byte"), (dict(d_v=FAKE + 2), "16-byte"),
+             (dict(n_pages=2**20, page_size=2**10, n_head_kv=4), "2^31")]
 BAD_SEQS = [(dict(n_seq=-1), "number of sequences"), (dict(max_pages=0), "number of sequences"), (dict(d_table=None), "NULL"), (dict(d_len=None), "NULL"),
             (dict(table_stride=3), "overlap"), (dict(max_pages=2**27, table_stride=2**27), "2^30")]
 
@@ -85,7 +86,7 @@ def test_bad_sequences_are_refused(pkg, bad, text):
     (dict(dtype=3), "dtype"), (dict(n_rows=4), "row_start"), (dict(d_k=None), "NULL"), (dict(d_v=None), "NULL"), (dict(n_head=0), "go together"),
     (dict(d_q=None), "go together"), (dict(d_q_out=None), "go together"), (dict(k_stride=199), "overlap"), (dict(v_stride=10), "overlap"),
     (dict(q_stride=399), "overlap"), (dict(q_out_stride=0), "overlap"), (dict(q_stride=500), "one stride"), (dict(d_k=FAKE + 2), "misaligned"),
-    (dict(d_rope_sin=None), "tables go together"), (dict(rope_ctx=0), "empty rope"), (dict(n_rows=2**31, d_row_start=FAKE), "2^31"), (dict(), "engine is NULL")])
+    (dict(d_rope_sin=None), "tables go together"), (dict(rope_ctx=0), "empty rope"), (dict(n_rows=2**31, d_row_start=FAKE), "2^30"), (dict(), "engine is NULL")])
 def test_bad_tokens_are_refused(pkg, bad, text):
     lib = pkg.lib()
     _refused(pkg, lib.nnb_paged_append(None, C.byref(_cache(pkg)), C.byref(_seqs(pkg)), C.byref(_tokens(pkg, **bad)), FAKE), text)

@@ -320,6 +320,28 @@ def test_append_ragged_prompts(pkg, eng, new, io, cache_dtype):
         assert torch.equal(vc[p, :, s], v[r + 2].to(cache_dtype).cpu())
 
 
+@pytest.mark.parametrize("heads,hk,dk,n,io", [(64, 8, 256, 5, F32), (128, 1, 128, 700, F32), (8, 2, 100, 2500, BF16), (7, 1, 34, 3000, F32), (2, 1, 50, 900, BF16)])
+def test_append_many_and_wide_tokens(pkg, eng, heads, hk, dk, n, io):
+    """Rows too wide for shared memory, odd head sizes, and enough tokens for several per CTA (the last CTA partly filled)."""
+    lens = [(7 * i) % 13 for i in range(n)]
+    cache, table, lengths = _pool(pkg, eng, lens, hk, 16, dk, BF16, room=1)
+    qkv = torch.randn((n, heads + 2 * hk, dk), device=eng.device).to(io)
+    q, k, v = qkv.split([heads, hk, hk], 1)
+    cos, sin = _tables(eng, dk, 16)
+    got_q, new = eng.paged_append(cache, table, lengths, k, v, q=q, rope=(cos, sin))
+    eng.check_device_errors()
+    at = lengths.long()
+    assert torch.equal(new, lengths + 1)
+    want, slack = _turned(q, cos[at], sin[at])
+    assert _near(got_q, want, slack)
+    want, slack = _turned(k, cos[at], sin[at])
+    rows = torch.arange(n, device=eng.device)
+    page = table[rows, at // 16].long()
+    assert _near(cache.k[page, :, at % 16, :dk], want, slack)
+    assert torch.equal(cache.v[page, :, at % 16, :dk], v.to(BF16))
+    assert not cache.k[page, :, at % 16, dk:].any() and not cache.v[page, :, at % 16, dk:].any()
+
+
 def test_append_without_queries_rotation_or_alignment(pkg, eng):
     lens, hk, dk = [3, 9], 2, 64
     for io, cache_dtype in ((F32, F32), (BF16, BF16)):
@@ -720,6 +742,26 @@ def test_captured_steps_follow_lengths_and_tables(pkg, eng):
             assert torch.equal(s["cache"].weight.nan_to_num(7.0), t["cache"].weight.nan_to_num(7.0))
             assert torch.equal(s["dst"].k, t["dst"].k)
     e2.close()
+
+
+def test_calls_follow_torchs_current_stream(pkg, eng):
+    """The engine launches on the default stream; a caller inside another stream's context gets its results in order."""
+    cache, table, lengths = _pool(pkg, eng, [600, 30], 2, 16, 64, BF16)
+    side = torch.cuda.Stream()
+    big = torch.randn((4096, 4096), device=eng.device)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        x = big
+        for _ in range(4):
+            x = (x @ big).clamp(-1, 1)
+        q = x.flatten()[:2 * 4 * 64].view(2, 4, 64).clone()
+        out, lse = eng.paged_attention_decode(cache, table, lengths, q)
+        y = eng.adjust_logits(out.view(2, -1), bias=out.view(2, -1)[0].contiguous())
+        got = [t.clone() for t in (q, out, lse, y)]
+    side.synchronize()
+    q, out, lse, y = got
+    _check_decode(cache, table, [600, 30], q, out, lse)
+    assert torch.equal(y, out.view(2, -1) + out.view(2, -1)[0])
 
 
 def test_an_engine_on_its_own_stream_is_ordered_with_torchs(pkg):
