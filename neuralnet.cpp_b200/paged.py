@@ -55,8 +55,8 @@ class PagedCache:
         if k.shape[3] != (dk + 7) // 8 * 8:
             raise NnbError(f"a head size of {dk} needs rows of {(dk + 7) // 8 * 8} features, not {k.shape[3]}")
         _need(weight is None or (weight.shape == k.shape[:3] and weight.dtype == torch.float32), "weights are (n_pages, n_head_kv, page_size) f32")
-        for t in (k, v) if weight is None else (k, v, weight):
-            _need(t.is_cuda and t.is_contiguous() and t.device == k.device, "the cache consists of contiguous CUDA tensors of one device")
+        _need(k.is_cuda and k.is_contiguous() and v.is_contiguous() and v.device == k.device
+              and (weight is None or (weight.is_contiguous() and weight.device == k.device)), "the cache consists of contiguous CUDA tensors of one device")
         self.k, self.v, self.weight, self.dk = k, v, weight, dk
         self.n_pages, self.n_head_kv, self.page_size, self.pitch = k.shape
         self._c = _Cache(k.data_ptr(), v.data_ptr(), weight.data_ptr() if weight is not None else None, _DTYPES[k.dtype], self.n_pages,
@@ -90,45 +90,53 @@ def _call(eng, fn, *args):
         cur.wait_stream(own)
 
 
-# The checks below run on every call: messages are only put together when one fails.
-def _on(eng, name, t, dtype, shape=None):
+# The checks below run on every call: one condition each, and messages only once it fails.
+def _wrong(eng, name, t, dtype, shape):
     if t.device != eng.device:
-        raise NnbError(f"{name} is on {t.device}, the engine on {eng.device}")
+        return NnbError(f"{name} is on {t.device}, the engine on {eng.device}")
     if t.dtype != dtype:
-        raise NnbError(f"{name} is {t.dtype}, not {dtype}")
+        return NnbError(f"{name} is {t.dtype}, not {dtype}")
     if shape is not None and t.shape != shape:
-        raise NnbError(f"{name} has shape {tuple(t.shape)}, not {shape}")
-    return t
+        return NnbError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+    return NnbError(f"{name} is not contiguous")
 
 
 def _flat(eng, name, t, dtype, shape):
-    if not _on(eng, name, t, dtype, shape).is_contiguous():
-        raise NnbError(f"{name} is not contiguous")
-    return t.data_ptr()
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.device == eng.device:
+        return t.data_ptr()
+    raise _wrong(eng, name, t, dtype, shape)
 
 
-def _rows(eng, name, t, heads=None, dk=None):
+def _matrix(eng, name, t, dtype):
+    """(rows, cols) with contiguous rows"""
+    if t.dim() == 2 and t.dtype is dtype and t.device == eng.device and (t.stride(1) == 1 or t.numel() == 0):
+        return t.shape
+    raise _wrong(eng, name, t, dtype, None) if t.dtype != dtype or t.device != eng.device else NnbError(f"{name} is a matrix with contiguous rows")
+
+
+def _rows(eng, name, t, heads, dk, dtype):
     """(rows, heads, dk) with contiguous rows, any distance apart; returns the distance in elements."""
-    if t.device != eng.device:
-        raise NnbError(f"{name} is on {t.device}, the engine on {eng.device}")
     shape = t.shape
-    if len(shape) != 3 or t.dtype not in _DTYPES:
-        raise NnbError(f"{name} is a (rows, heads, dk) tensor, f32 or bf16")
-    if (heads is not None and shape[1] != heads) or (dk is not None and shape[2] != dk):
-        raise NnbError(f"{name} has shape {tuple(shape)}")
-    row, head, one = t.stride()
-    if (one != 1 or (shape[1] != 1 and head != shape[2]) or row < 0) and t.numel():
+    if len(shape) == 3 and shape[1] == heads and shape[2] == dk and t.dtype is dtype and t.device == eng.device:
+        row, head, one = t.stride()
+        if (one == 1 and (head == dk or heads == 1) and row >= 0) or t.numel() == 0:
+            return row
         raise NnbError(f"the rows of {name} are not contiguous")
-    return row
+    raise _wrong(eng, name, t, dtype, (shape[0] if len(shape) else 0, heads, dk))
 
 
 def _seqs(eng, cache, table, lengths):
     if cache.k.device != eng.device:
         raise NnbError(f"the cache is on {cache.k.device}, the engine on {eng.device}")
-    if _on(eng, "table", table, torch.int32).dim() != 2 or (table.stride(1) != 1 and table.numel()):
-        raise NnbError("table is (n_seq, max_pages) with contiguous rows")
-    n, cols = table.shape
+    n, cols = _matrix(eng, "table", table, torch.int32)
     return _Seqs(table.data_ptr(), _flat(eng, "lengths", lengths, torch.int32, (n,)), n, cols, table.stride(0) if n > 1 else cols)
+
+
+def _heads(name, t):
+    """the heads of a (rows, heads, dk) tensor, f32 or bf16"""
+    if t.dim() != 3 or t.dtype not in _DTYPES:
+        raise NnbError(f"{name} is a (rows, heads, dk) tensor, f32 or bf16")
+    return t.shape[1]
 
 
 def paged_append(self, cache, table, lengths, k, v, q=None, row_start=None, rope=None, positions=None, q_out=None, lengths_out=None):
@@ -136,36 +144,39 @@ def paged_append(self, cache, table, lengths, k, v, q=None, row_start=None, rope
     positions (default: their place in the cache).  row_start (n_seq + 1): the rows of each sequence; None: one row per
     sequence, idle where its position is negative.  Returns (rotated q or None, new lengths); lengths_out may be lengths."""
     s = _seqs(self, cache, table, lengths)
-    rows, n = k.shape[0], s.n_seq
-    ks, vs = _rows(self, "k", k, cache.n_head_kv, cache.dk), _rows(self, "v", v, cache.n_head_kv, cache.dk)
-    if v.shape[0] != rows or v.dtype != k.dtype:
-        raise NnbError("k and v differ in rows or type")
-    t = _Tokens(None, k.data_ptr(), v.data_ptr(), None, 0, ks, vs, 0, _DTYPES[k.dtype], 0, rows, None, None, None, None, 0)
+    _heads("k", k)
+    rows, n, io, dk = k.shape[0], s.n_seq, k.dtype, cache.dk
+    ks, vs = _rows(self, "k", k, cache.n_head_kv, dk, io), _rows(self, "v", v, cache.n_head_kv, dk, io)
+    if v.shape[0] != rows or (q is not None and q.shape[0] != rows):
+        raise NnbError("q, k and v differ in rows")
+    qs = q_ptr = out_ptr = out_stride = heads = start = pos = cos_ptr = sin_ptr = ctx = 0
     if q is not None:
-        t.q_stride = _rows(self, "q", q, None, cache.dk)
-        if q.shape[0] != rows or q.dtype != k.dtype:
-            raise NnbError("q and k differ in rows or type")
+        heads = _heads("q", q)
+        qs, q_ptr = _rows(self, "q", q, heads, dk, io), q.data_ptr()
         if q_out is None:
-            q_out, t.q_out_stride = q.new_empty(q.shape), q.shape[1] * q.shape[2]
+            q_out, out_stride = torch.empty_like(q, memory_format=torch.contiguous_format), heads * dk
         else:
-            t.q_out_stride = _rows(self, "q_out", q_out)
-            if q_out.shape != q.shape or q_out.dtype != q.dtype:
-                raise NnbError("q_out and q differ in shape or type")
-        t.n_head, t.d_q, t.d_q_out = q.shape[1], q.data_ptr(), q_out.data_ptr()
+            out_stride = _rows(self, "q_out", q_out, heads, dk, io)
+            if q_out.shape[0] != rows:
+                raise NnbError("q_out and q differ in rows")
+        out_ptr = q_out.data_ptr()
     else:
         q_out = None
     if row_start is not None:
-        t.d_row_start = _flat(self, "row_start", row_start, torch.int32, (n + 1,))
+        start = _flat(self, "row_start", row_start, torch.int32, (n + 1,))
     if positions is not None:
-        t.d_pos = _flat(self, "positions", positions, torch.int32, (rows,))
+        pos = _flat(self, "positions", positions, torch.int32, (rows,))
     if rope is not None:
         cos, sin = rope
-        t.d_rope_cos = _flat(self, "cos", cos, torch.float32, (cos.shape[0], cache.dk // 2))
-        t.d_rope_sin, t.rope_ctx = _flat(self, "sin", sin, torch.float32, tuple(cos.shape)), cos.shape[0]
+        ctx = cos.shape[0]
+        cos_ptr, sin_ptr = _flat(self, "cos", cos, torch.float32, (ctx, dk // 2)), _flat(self, "sin", sin, torch.float32, (ctx, dk // 2))
     if lengths_out is None:
         lengths_out = torch.empty_like(lengths)
-    out = _flat(self, "lengths_out", lengths_out, torch.int32, (n,))
-    _call(self, self._lib.nnb_paged_append, C.byref(cache._c), C.byref(s), C.byref(t), out)
+        len_ptr = lengths_out.data_ptr()
+    else:
+        len_ptr = _flat(self, "lengths_out", lengths_out, torch.int32, (n,))
+    t = _Tokens(q_ptr, k.data_ptr(), v.data_ptr(), out_ptr, qs, ks, vs, out_stride, _DTYPES[io], heads, rows, start, pos, cos_ptr, sin_ptr, ctx)
+    _call(self, self._lib.nnb_paged_append, C.byref(cache._c), C.byref(s), C.byref(t), len_ptr)
     return q_out, lengths_out
 
 
@@ -173,23 +184,23 @@ def paged_attention_decode(self, cache, table, lengths, q, scale=0.0, accumulate
     """Attention of one new token per sequence, q (n_seq, n_head, dk), over the `lengths` cached positions.  Returns
     (out (n_seq, n_head, dk) of q's type, lse (n_seq, n_head) f32); accumulate adds the attention weights to cache.weight."""
     s = _seqs(self, cache, table, lengths)
-    stride = _rows(self, "q", q, None, cache.dk)
-    n, heads = s.n_seq, q.shape[1]
+    n, heads, io = s.n_seq, _heads("q", q), q.dtype
+    stride = _rows(self, "q", q, heads, cache.dk, io)
     if q.shape[0] != n:
         raise NnbError(f"{q.shape[0]} queries for {n} sequences")
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        _flat(self, "out", out, q.dtype, q.shape)
+        _flat(self, "out", out, io, q.shape)
     if lse is None:
-        lse = q.new_empty((n, heads), dtype=torch.float32)
+        lse = torch.empty((n, heads), device=self.device, dtype=torch.float32)
     else:
         _flat(self, "lse", lse, torch.float32, (n, heads))
-    accumulate, d_out, d_lse = int(accumulate), out.data_ptr(), lse.data_ptr()
-    size = self._lib.nnb_paged_attention_workspace(self._h, C.byref(cache._c), C.byref(s), heads, accumulate)
-    ws = q.new_empty(size, dtype=torch.uint8)
-    _call(self, self._lib.nnb_paged_attention_decode, C.byref(cache._c), C.byref(s), q.data_ptr(), _DTYPES[q.dtype], stride, heads, scale, d_out, d_lse,
-          accumulate, ws.data_ptr(), size)
+    accumulate, c, s = int(accumulate), C.byref(cache._c), C.byref(s)
+    size = self._lib.nnb_paged_attention_workspace(self._h, c, s, heads, accumulate)
+    ws = torch.empty(size, device=self.device, dtype=torch.uint8)
+    _call(self, self._lib.nnb_paged_attention_decode, c, s, q.data_ptr(), _DTYPES[io], stride, heads, scale, out.data_ptr(), lse.data_ptr(), accumulate,
+          ws.data_ptr(), size)
     return out, lse
 
 
@@ -203,7 +214,7 @@ def paged_evict(self, cache, table, lengths, dst, dst_table, budget, sinks=0, re
     n_out = _flat(self, "lengths_out", lengths_out, torch.int32, (s.n_seq,))
     _need(budget >= 0 and sinks >= 0 and recent >= 0, "budget, sinks and recent are not negative")
     size = self._lib.nnb_paged_evict_workspace(self._h, C.byref(cache._c), C.byref(s), budget)
-    ws = lengths.new_empty(size, dtype=torch.uint8)
+    ws = torch.empty(size, device=self.device, dtype=torch.uint8)
     _call(self, self._lib.nnb_paged_evict, C.byref(cache._c), C.byref(s), budget, sinks, recent, C.byref(dst._c), d.d_table, d.max_pages, d.table_stride,
           n_out, ws.data_ptr(), size)
     return lengths_out
@@ -214,34 +225,34 @@ def adjust_logits(self, logits, history=None, history_len=None, prompt_len=None,
     """logits (n_seq, vocab) f32 or bf16 with a bias, penalties for the ids of history (n_seq, max_history) and a mask of
     allowed ids (one bit each, (n_seq, ceil(vocab / 32)) int32), in this order.  Penalties are (n_seq) f32, bias and allowed
     one row for all or one per sequence; out may be logits.  Returns out."""
-    _need(logits.dim() == 2 and logits.dtype in _DTYPES and logits.device == self.device, "logits is an (n_seq, vocab) tensor on the engine's device, f32 or bf16")
-    n, vocab = logits.shape
+    io = logits.dtype
+    if io not in _DTYPES:
+        raise NnbError("logits are f32 or bf16")
+    n, vocab = _matrix(self, "logits", logits, io)
     if out is None:
-        out = logits.new_empty((n, vocab))
-    else:
-        _on(self, "out", out, logits.dtype, (n, vocab))
-    _need(n == 0 or (logits.stride(1) == 1 and out.stride(1) == 1), "rows of the logits are not contiguous")
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    elif _matrix(self, "out", out, io) != logits.shape:
+        raise NnbError(f"out has shape {tuple(out.shape)}, not {tuple(logits.shape)}")
     c = _Logits()
     c.repeat_window = repeat_window
-    penalties = (("d_repeat", "repeat_penalty", repeat_penalty), ("d_presence", "presence_penalty", presence_penalty),
-                 ("d_frequency", "frequency_penalty", frequency_penalty))
     if history is None:
-        _need(all(t is None for _, _, t in penalties), "penalties need a history")
+        _need(repeat_penalty is None and presence_penalty is None and frequency_penalty is None, "penalties need a history")
     else:
-        _need(_on(self, "history", history, torch.int32).dim() == 2 and history.shape[0] == n and (history.numel() == 0 or history.stride(1) == 1),
-              "history is (n_seq, max_history) with contiguous rows")
-        _need(history_len is not None, "history needs history_len")
-        given = [(field, _flat(self, name, t, torch.float32, (n,))) for field, name, t in penalties if t is not None]
-        lens = _flat(self, "history_len", history_len, torch.int32, (n,))
-        prompt = _flat(self, "prompt_len", prompt_len, torch.int32, (n,)) if prompt_len is not None else None
-        if history.numel():  # with an empty one there is nothing to penalise
-            c.d_history, c.history_stride, c.max_history = history.data_ptr(), history.stride(0), history.shape[1]
-            c.d_history_len, c.d_prompt_len = lens, prompt
-            for field, ptr in given:
-                setattr(c, field, ptr)
+        rows, width = _matrix(self, "history", history, torch.int32)
+        _need(rows == n and history_len is not None, "history has a row and a length for every sequence")
+        f32, one = torch.float32, (n,)
+        lens = _flat(self, "history_len", history_len, torch.int32, one)
+        prompt = _flat(self, "prompt_len", prompt_len, torch.int32, one) if prompt_len is not None else 0
+        rep = _flat(self, "repeat_penalty", repeat_penalty, f32, one) if repeat_penalty is not None else 0
+        pres = _flat(self, "presence_penalty", presence_penalty, f32, one) if presence_penalty is not None else 0
+        freq = _flat(self, "frequency_penalty", frequency_penalty, f32, one) if frequency_penalty is not None else 0
+        if rows * width:  # with an empty one there is nothing to penalise
+            c.d_history, c.history_stride, c.max_history, c.d_history_len = history.data_ptr(), history.stride(0), width, lens
+            c.d_prompt_len, c.d_repeat, c.d_presence, c.d_frequency = prompt, rep, pres, freq
     for name, t, dtype, width in (("bias", bias, torch.float32, vocab), ("allowed", allowed, torch.int32, (vocab + 31) // 32)):
         if t is not None:
-            _on(self, name, t, dtype)
+            if t.dtype != dtype or t.device != self.device:
+                raise _wrong(self, name, t, dtype, None)
             if tuple(t.shape) not in ((width,), (n, width)) or t.stride(-1) != 1:
                 raise NnbError(f"{name} is ({width}) or ({n}, {width}) with contiguous rows")
             setattr(c, "d_" + name, t.data_ptr())
