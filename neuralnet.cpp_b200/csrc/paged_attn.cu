@@ -1,4 +1,5 @@
 // paged_attn.cu — attention of one new token per sequence over a paged key-value cache.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include "device_math.cuh"
@@ -31,6 +32,10 @@ __device__ __forceinline__ void store_one(__nv_bfloat16* p, float x) { *p = __fl
 // items that lie inside its range; of an item that several workers share each leaves a partial softmax (maximum, sum,
 // weighted values) that paged_join_kernel folds in order.  A worker has at most two partial items: slot 0 is one that began
 // in an earlier worker, slot 1 one that begins here and goes on in the next.
+//
+// A short call (few items over a short table) is dealt out differently, to a cluster of CLUSTER CTAs per item, which share its
+// tiles evenly and join through distributed shared memory: one launch less, and no way through global memory.
+constexpr int CLUSTER = 8, SHORT_CALL = 2048;  // the longest table of a short call, in positions
 constexpr int LONG_CALL = 96;  // units per worker from which on a call has a second set of workers
 constexpr int MAX_CTAS_PER_SM = 4, MAX_WORKERS = MAX_CTAS_PER_SM * 3 / 2 /* per SM, both sets */, MAX_UNIT = 64, ITEM_COST = 2;
 
@@ -42,6 +47,7 @@ struct DecodeWs {
     float* scores;   // (n_seq, n_head, score_stride): scores in the log2 domain, for the weights; or NULL
     long long score_stride;
     int wh, wide;    // wide: workers of the first set
+    int clusters;    // a short call
     int rows, dkm;   // query heads of an item per KV head, and the pitch of the partial results
     int slab_groups; // items per (sequence, wh KV heads): larger groups of query heads than a pass serves are cut
 };
@@ -84,6 +90,18 @@ struct Deal {
         return u < head ? (int)(((u + 1) * wide - 1) / head) : wide + (int)(((u - head + 1) * rest - 1) / (units - head));
     }
 };
+
+// the same for a short call: this CTA's tiles of its cluster's item
+__device__ __forceinline__ bool find_tiles(const PagedView& c, const SeqView& s, int unit, int items_per_seq, UnitIter& it, long long& left, int* flags)
+{
+    const int item = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;
+    it.seq = item / items_per_seq;
+    it.hs = item % items_per_seq;
+    load_seq(it, c, s, unit, flags);
+    it.tile = it.tiles * rank / CLUSTER;
+    left = it.tiles * (rank + 1) / CLUSTER - it.tile;
+    return left > 0;
+}
 
 // Called by all 128 threads: this worker's range of the cost and the place of its first unit; false if it has none.
 __device__ __forceinline__ bool find_work(const PagedView& c, const SeqView& s, int unit, int items_per_seq, const DecodeWs& ws, UnitIter& it, long long& u0, long long& u1,
@@ -228,10 +246,10 @@ __device__ __forceinline__ void prefetch_queries(const PagedView& c, const Decod
 }
 
 // Folds the results that the wp warps of a KV head have parked (rows of STRIDE floats, then maximum and sum per row; warps
-// warp_stride floats apart) and writes them: outputs if the item is whole, a partial result otherwise.
+// warp_stride floats apart) and writes them: outputs if the item is whole, a partial result (to part, part_ml) otherwise.
 template <int DKM, int STRIDE, int ROWS, typename TQ>
 __device__ __forceinline__ void fold_warps(const float* parked, int warp_stride, int wp, const PagedView& c, const DecodeArgs& a, const DecodeWs& ws,
-                                           int seq, int hk, int row0, bool whole, int slot)
+                                           int seq, int hk, int row0, bool whole, float* part, float* part_ml)
 {
     const int rows = min(min(ROWS, ws.rows), a.group - row0), threads = 32 * wp, in_head = (threadIdx.x >> 5) / wp;
     for (int p = threadIdx.x & (threads - 1); p < rows * (DKM / 4); p += threads) {
@@ -262,11 +280,66 @@ __device__ __forceinline__ void fold_warps(const float* parked, int warp_stride,
                 if (ws.lse2) ws.lse2[hq] = z;
             }
         } else {
-            const long long pr = (((long long)blockIdx.x * 2 + slot) * ws.wh + in_head) * ws.rows + r;
-            *reinterpret_cast<float4*>(ws.o + pr * ws.dkm + f) = x;
-            if (f == 0) *reinterpret_cast<float2*>(ws.ml + pr * 2) = make_float2(top, sum);
+            const int pr = in_head * ws.rows + r;
+            *reinterpret_cast<float4*>(part + pr * ws.dkm + f) = x;
+            if (f == 0) *reinterpret_cast<float2*>(part_ml + pr * 2) = make_float2(top, sum);
         }
     }
+}
+
+// Short calls: a CTA's partial result of its item in shared memory, empty at first: (wh, rows, dkm) values, then (wh, rows)
+// maximum and sum.
+__device__ __forceinline__ void clear_partial(float* part, const DecodeWs& ws)
+{
+    float2* ml = reinterpret_cast<float2*>(part + ws.wh * ws.rows * ws.dkm);
+    for (int i = threadIdx.x; i < ws.wh * ws.rows; i += 128) ml[i] = make_float2(-INFINITY, 0.0f);
+}
+// The CTAs of the cluster fold their partial results, each for its share of the values, in the order of their ranks.
+template <typename TQ>
+__device__ void join_cluster(float* part, const PagedView& c, const DecodeArgs& a, const DecodeWs& ws, int seq, int hs)
+{
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int rank = (int)cluster.block_rank(), vecs = ws.dkm / 4;
+    float* ml = part + ws.wh * ws.rows * ws.dkm;
+    for (int p = rank * 128 + threadIdx.x; p < ws.wh * ws.rows * vecs; p += CLUSTER * 128) {
+        const int row = p / vecs, f = (p - row * vecs) * 4;
+        const int gi = hs % ws.slab_groups * ws.rows + row % ws.rows, hk = hs / ws.slab_groups * ws.wh + row / ws.rows;
+        if (gi >= a.group) continue;
+        float2 m[CLUSTER];
+        float4 y[CLUSTER];
+#pragma unroll
+        for (int r = 0; r < CLUSTER; ++r) m[r] = *reinterpret_cast<const float2*>(cluster.map_shared_rank(ml + 2 * row, r));
+#pragma unroll
+        for (int r = 0; r < CLUSTER; ++r)  // (the values of a CTA without any tile were never written)
+            y[r] = m[r].x == -INFINITY ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *reinterpret_cast<const float4*>(cluster.map_shared_rank(part + row * ws.dkm + f, r));
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < CLUSTER; ++r) top = fmaxf(top, m[r].x);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int r = 0; r < CLUSTER; ++r) {
+            const float k = exp2f(m[r].x - base);
+            sum = fmaf(m[r].y, k, sum);
+            x[0] = fmaf(y[r].x, k, x[0]);
+            x[1] = fmaf(y[r].y, k, x[1]);
+            x[2] = fmaf(y[r].z, k, x[2]);
+            x[3] = fmaf(y[r].w, k, x[3]);
+        }
+        const long long hq = (long long)seq * a.n_head + hk * a.group + gi;
+        const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (f + i < c.dk) store_one((TQ*)a.out + hq * c.dk + f + i, x[i] * inv);
+        if (f == 0) {
+            const float z = sum == 0.0f ? -INFINITY : top + log2f(sum);
+            if (a.lse) a.lse[hq] = z * 0.693147180559945309f;
+            if (ws.lse2) ws.lse2[hq] = z;
+        }
+    }
+    cluster.sync();  // nobody leaves while its shared memory is read
 }
 
 // ------------------------------------------------------------------------------------------------ bf16 caches
@@ -306,17 +379,26 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     __nv_bfloat16* ring = reinterpret_cast<__nv_bfloat16*>(smem_raw) + (size_t)warp * NST * C::STAGE;
     __nv_bfloat16* qs = reinterpret_cast<__nv_bfloat16*>(smem_raw) + (size_t)4 * NST * C::STAGE + (size_t)(warp / (4 / ws.wh)) * C::QROWS * LD;
+    float* shared_part = reinterpret_cast<float*>(smem_raw + C::SMEM);  // of a short call
     pdl_wait();
     pdl_launch();
     const int wp = 4 / ws.wh, unit = TK * wp, in_head = warp / wp, items_per_seq = c.heads / ws.wh * ws.slab_groups;
     UnitIter ct;
-    long long u_begin, u_end;
+    long long u_begin, u_end, left;  // left: cost for the computing side
     Deal deal;
-    const bool work = find_work(c, s, unit, items_per_seq, ws, ct, u_begin, u_end, deal, flags);
-    if (tid == 0) ws.desc[blockIdx.x] = make_int2(-1, -1);
-    if (!work) return;
-    // cost left for the computing and for the issuing side, which runs NST units ahead
-    long long left = u_end - u_begin, to_issue = left;
+    if (ws.clusters) {
+        clear_partial(shared_part, ws);
+        if (!find_tiles(c, s, unit, items_per_seq, ct, left, flags)) {
+            join_cluster<TQ>(shared_part, c, a, ws, ct.seq, ct.hs);
+            return;
+        }
+    } else {
+        const bool work = find_work(c, s, unit, items_per_seq, ws, ct, u_begin, u_end, deal, flags);
+        if (tid == 0) ws.desc[blockIdx.x] = make_int2(-1, -1);
+        if (!work) return;
+        left = u_end - u_begin;
+    }
+    long long to_issue = left;  // for the issuing side, which runs NST units ahead
 
     const char* kbase = (const char*)c.k;
     const char* vbase = (const char*)c.v;
@@ -614,8 +696,8 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
         }
         __syncwarp();
         if (closing) {  // fold the four warps' results
-            const bool whole = starts_here && ends;
-            if (tid == 0 && starts_here && !ends)
+            const bool whole = starts_here && ends && !ws.clusters;
+            if (tid == 0 && starts_here && !ends && !ws.clusters)
                 ws.desc[blockIdx.x] = make_int2(ct.seq * items_per_seq + ct.hs, deal.worker_of(u_end - 1 + (ct.tiles - 1 - ct.tile)));
             float* park = reinterpret_cast<float*>(ring + stage * C::STAGE);
 #pragma unroll
@@ -637,8 +719,11 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
                 if (t4 == 0) *reinterpret_cast<float2*>(park + C::ROWS * C::PARK + (sl * 8 + g) * 2) = make_float2(m[sl], ls);
             }
             __syncthreads();
+            const long long part_row = ((long long)blockIdx.x * 2 + (starts_here ? 1 : 0)) * ws.wh * ws.rows;
+            float* part = ws.clusters ? shared_part : ws.o + part_row * ws.dkm;
+            float* part_ml = ws.clusters ? shared_part + ws.wh * ws.rows * ws.dkm : ws.ml + part_row * 2;
             fold_warps<C::DKM, C::PARK, C::ROWS, TQ>(reinterpret_cast<const float*>(smem_raw) + (in_head * wp * NST + stage) * (C::STAGE / 2),
-                                                     NST * (C::STAGE / 2), wp, c, a, ws, ct.seq, hk, row0, whole, starts_here ? 1 : 0);
+                                                     NST * (C::STAGE / 2), wp, c, a, ws, ct.seq, hk, row0, whole, part, part_ml);
             __syncthreads();
             fresh = true;
         }
@@ -649,6 +734,7 @@ paged_decode_mma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
         if (++ct.tile == ct.tiles) next_item(ct, c, s, unit, items_per_seq, flags);
     }
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+    if (ws.clusters) join_cluster<TQ>(shared_part, c, a, ws, ct.seq, ct.hs);
 }
 
 // ------------------------------------------------------------------------------------------------ f32 caches
@@ -675,18 +761,28 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
     extern __shared__ __align__(16) float smem_f[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ld = C::ld(c.pitch), stage_len = 2 * TK * ld;
     float* ring = smem_f + (size_t)warp * NST * stage_len;
+    float* shared_part = smem_f + C::smem(C::DKM) / sizeof(float);  // of a short call
     pdl_wait();
     pdl_launch();
     const int wp = 4 / ws.wh, unit = TK * wp, in_head = warp / wp, items_per_seq = c.heads / ws.wh * ws.slab_groups;
     float* qs = smem_f + (size_t)4 * NST * stage_len + (size_t)in_head * ROWS * ld;  // one copy per KV head of the CTA
     float* ps = smem_f + (size_t)4 * NST * stage_len + (size_t)ws.wh * ROWS * ld + warp * TK * ROWS;  // this warp's probabilities, (position, row)
     UnitIter ct;
-    long long u_begin, u_end;
+    long long u_begin, u_end, left;
     Deal deal;
-    const bool work = find_work(c, s, unit, items_per_seq, ws, ct, u_begin, u_end, deal, flags);
-    if (tid == 0) ws.desc[blockIdx.x] = make_int2(-1, -1);
-    if (!work) return;
-    long long left = u_end - u_begin, to_issue = left;
+    if (ws.clusters) {
+        clear_partial(shared_part, ws);
+        if (!find_tiles(c, s, unit, items_per_seq, ct, left, flags)) {
+            join_cluster<TQ>(shared_part, c, a, ws, ct.seq, ct.hs);
+            return;
+        }
+    } else {
+        const bool work = find_work(c, s, unit, items_per_seq, ws, ct, u_begin, u_end, deal, flags);
+        if (tid == 0) ws.desc[blockIdx.x] = make_int2(-1, -1);
+        if (!work) return;
+        left = u_end - u_begin;
+    }
+    long long to_issue = left;
 
     const int chunks = c.pitch / 4, key = lane / LPK, sub = lane % LPK;
     const float* kbase = (const float*)c.k;
@@ -859,8 +955,8 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
         left -= ends ? 1 + ITEM_COST : 1;
         const bool last = left <= 0;
         if (ends || last) {  // fold the lanes' and the warps' results
-            const bool whole = starts_here && ends;
-            if (tid == 0 && starts_here && !ends)
+            const bool whole = starts_here && ends && !ws.clusters;
+            if (tid == 0 && starts_here && !ends && !ws.clusters)
                 ws.desc[blockIdx.x] = make_int2(ct.seq * items_per_seq + ct.hs, deal.worker_of(u_end - 1 + (ct.tiles - 1 - ct.tile)));
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
@@ -887,8 +983,11 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
                 }
             }
             __syncthreads();
-            fold_warps<C::DKM, C::DKM, ROWS, TQ>(smem_f + (in_head * wp * NST + stage) * stage_len, NST * stage_len, wp, c, a, ws, ct.seq, hk, row0, whole,
-                                                 starts_here ? 1 : 0);
+            const long long part_row = ((long long)blockIdx.x * 2 + (starts_here ? 1 : 0)) * ws.wh * ws.rows;
+            float* part = ws.clusters ? shared_part : ws.o + part_row * ws.dkm;
+            float* part_ml = ws.clusters ? shared_part + ws.wh * ws.rows * ws.dkm : ws.ml + part_row * 2;
+            fold_warps<C::DKM, C::DKM, ROWS, TQ>(smem_f + (in_head * wp * NST + stage) * stage_len, NST * stage_len, wp, c, a, ws, ct.seq, hk, row0, whole, part,
+                                                 part_ml);
             __syncthreads();
             fresh = true;
         }
@@ -898,6 +997,7 @@ paged_decode_fma_kernel(const PagedView c, const SeqView s, const DecodeArgs a, 
         if (++ct.tile == ct.tiles) next_item(ct, c, s, unit, items_per_seq, flags);
     }
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+    if (ws.clusters) join_cluster<TQ>(shared_part, c, a, ws, ct.seq, ct.hs);
 }
 
 // ------------------------------------------------------------------------------------------------ joining
@@ -1036,15 +1136,37 @@ template <typename... K>
 static nnb_status launch_workers(nnb_engine* e, void (*kern)(K...), size_t smem, int (&per_sm)[64], const PagedView& c, const SeqView& s, const DecodeArgs& a,
                                  DecodeWs ws, int* workers)
 {
+    const size_t part = (size_t)ws.wh * ws.rows * (ws.dkm + 2) * sizeof(float);
     int& n = per_sm[e->device & 63];  // resident CTAs per SM, by device
-    if (n == 0) {
-        NNB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (n == 0) {  // (a short call's parts: at most 16 rows)
+        NNB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(smem + 16 * (ws.dkm + 2) * sizeof(float))));
         NNB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, 128, smem));
         n = n < 1 ? 1 : n > MAX_CTAS_PER_SM ? MAX_CTAS_PER_SM : n;
     }
     ws.wide = e->sm_count * n;
+    const size_t items = (size_t)s.n_seq * (c.heads / ws.wh) * ws.slab_groups, cap = (size_t)paged_capacity(c, s);
+    // One CTA per SM at most, so that the clusters of a short call find room at once.
+    if (cap <= SHORT_CALL && items * CLUSTER <= (size_t)e->sm_count) {
+        ws.clusters = 1;
+        *workers = 0;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)items * CLUSTER);
+        cfg.blockDim = dim3(128);
+        cfg.dynamicSmemBytes = smem + part;
+        cfg.stream = e->stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim = {CLUSTER, 1, 1};
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+        NNB_CUDA(cudaLaunchKernelEx(&cfg, kern, c, s, a, ws, e->dev_flags));
+        e->launches++;
+        return NNB_OK;
+    }
     // (the lengths are on the device: the table's capacity bounds the cost from above)
-    const size_t unit = 16 * (4 / ws.wh), most = (size_t)s.n_seq * (c.heads / ws.wh) * ws.slab_groups * (ceil_div((size_t)paged_capacity(c, s), unit) + ITEM_COST);
+    const size_t most = items * (ceil_div(cap, (size_t)16 * (4 / ws.wh)) + ITEM_COST);
     *workers = most >= (size_t)LONG_CALL * ws.wide ? ws.wide + ws.wide / 2 : ws.wide;
     NNB_CUDA(launch_ex(e, kern, dim3((unsigned)*workers), dim3(128), smem, c, s, a, ws, e->dev_flags));
     e->launches++;
@@ -1083,7 +1205,7 @@ static nnb_status launch_decode(nnb_engine* e, bool f32_cache, const PagedView& 
 {
     const WsPlan p = plan_ws(e->sm_count, f32_cache, c, s, (size_t)a.n_head, accumulate);
     DecodeWs ws{(int2*)(base + p.desc), (float*)(base + p.ml), (float*)(base + p.o), accumulate ? (float*)(base + p.lse2) : nullptr,
-                      accumulate ? (float*)(base + p.scores) : nullptr, p.score_stride, p.wh, 0, p.rows, p.dkm, p.slab_groups};
+                      accumulate ? (float*)(base + p.scores) : nullptr, p.score_stride, p.wh, 0, 0, p.rows, p.dkm, p.slab_groups};
     PdlOn pdl(e);
     int workers = 0;
     if (f32_cache) {
@@ -1102,10 +1224,11 @@ static nnb_status launch_decode(nnb_engine* e, bool f32_cache, const PagedView& 
             default: NNB_TRY((launch_mma<16, TQ>(e, c, s, a, ws, &workers))); break;
         }
     }
-    const size_t smem = (size_t)(workers > 512 ? workers : 512) * sizeof(float);
-    NNB_CUDA(launch_ex(e, paged_join_kernel<TQ>, dim3((unsigned)workers, (unsigned)(p.wh * p.rows)), dim3(128), smem, c, s, a, ws,
-                       e->dev_flags));
-    e->launches++;
+    if (workers > 0) {  // (a short call has joined its parts itself)
+        const size_t smem = (size_t)(workers > 512 ? workers : 512) * sizeof(float);
+        NNB_CUDA(launch_ex(e, paged_join_kernel<TQ>, dim3((unsigned)workers, (unsigned)(p.wh * p.rows)), dim3(128), smem, c, s, a, ws, e->dev_flags));
+        e->launches++;
+    }
     if (accumulate) {
         const unsigned items = (unsigned)(s.n_seq * c.heads);
         const size_t want = ceil_div((size_t)e->sm_count * 8, items), most = ceil_div((size_t)paged_capacity(c, s), 256);
