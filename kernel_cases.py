@@ -15,6 +15,8 @@ Used for Nsight Compute captures and quick timing; every case prints its CUDA-ev
                default 128 16 48); `layers` cuts the depth (same kernels, less memory: for profiler captures)
   rollout2b4t [B P new [layers]] the same on the BitNet-b1.58-2B4T structure (30 layers, d 2560, 20 heads on 5 KV heads of
                128, SubLN, ReLU2GLU, tied embeddings, vocab 128256)
+  paged [n len] one step of n (64) sequences of len (4000) positions on a paged cache, 32 heads on 8 KV heads of 128:
+               append, decode attention with accumulated weights, eviction to a quarter, logit adjustment (vocab 128256)
   lmhead [T]   LM head fused with log-prob / entropy, forward and backward, T (8192) decisions x d 2048 x vocab 32000
 """
 import os
@@ -75,6 +77,31 @@ def main(argv):
     pkg = load_package()
     eng = pkg.Engine(0)
     dev = eng.device
+    if case == "paged":
+        n, length = int(argv[2]) if len(argv) > 2 else 64, int(argv[3]) if len(argv) > 3 else 4000
+        pages = (length + 64) // 64
+        cache = pkg.PagedCache.empty(n * pages, 8, 64, 128, device=dev, track_weight=True)
+        cache.k.normal_()
+        cache.v.normal_()
+        cache.weight.uniform_()
+        table = torch.randperm(n * pages, device=dev).int().view(n, pages)
+        lengths = torch.full((n,), length, dtype=torch.int32, device=dev)
+        q, k, v = torch.randn((n, 48, 128), device=dev, dtype=torch.bfloat16).split([32, 8, 8], 1)
+        cos, sin = torch.empty((length + 1, 64), device=dev), torch.empty((length + 1, 64), device=dev)
+        ang = torch.arange(length + 1, device=dev)[:, None] * 10000.0 ** (-torch.arange(64, device=dev) / 64)
+        cos.copy_(ang.cos())
+        sin.copy_(ang.sin())
+        dst = pkg.PagedCache.empty(n * ((length // 4 + 63) // 64), 8, 64, 128, device=dev, track_weight=True)
+        dst_table = torch.arange(dst.n_pages, dtype=torch.int32, device=dev).view(n, -1)
+        logits, history = torch.randn((n, 128256), device=dev), torch.randint(0, 128256, (n, 2048), dtype=torch.int32, device=dev)
+        hist_len, penalty = torch.full((n,), 2048, dtype=torch.int32, device=dev), torch.full((n,), 1.2, device=dev)
+        _timed("append", lambda: eng.paged_append(cache, table, lengths, k, v, q=q, rope=(cos, sin)))
+        _timed("decode", lambda: eng.paged_attention_decode(cache, table, lengths, q))
+        _timed("decode, weights", lambda: eng.paged_attention_decode(cache, table, lengths, q, accumulate=True))
+        _timed("evict", lambda: eng.paged_evict(cache, table, lengths, dst, dst_table, budget=length // 4, sinks=4, recent=length // 16))
+        _timed("adjust_logits", lambda: eng.adjust_logits(logits, history=history, history_len=hist_len, repeat_penalty=penalty))
+        eng.check_device_errors()
+        return
     if case in ("fwd", "dx", "dw"):
         T, k, out = 10240, 2048, 11264
         w8, wb = eng.expand_weights(_rand_packed(dev, out, k // 16), k)

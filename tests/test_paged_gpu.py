@@ -110,6 +110,15 @@ def test_decode_of_long_contexts_is_split_and_joined(pkg, eng, lens, heads, hk, 
     _decode(pkg, eng, lens, heads, hk, page, dk, cache_dtype, io, seed=len(lens))
 
 
+@pytest.mark.parametrize("cache_dtype,io", [(BF16, F32), (BF16, BF16), (F32, F32)])
+@pytest.mark.parametrize("heads,hk,page,dk", [(3, 1, 3, 8), (8, 1, 16, 2), (8, 4, 16, 16), (4, 2, 8, 72), (5, 5, 16, 136)])
+def test_decode_of_more_sequences_than_workers(pkg, eng, heads, hk, page, dk, cache_dtype, io):
+    """Several short sequences per worker, empty ones among them, and narrow rows (a tile smaller than a result)."""
+    rng = np.random.default_rng(dk)
+    lens = [int(x) for x in rng.integers(0, 40, 700) * (rng.random(700) > 0.1)]
+    _decode(pkg, eng, lens, heads, hk, page, dk, cache_dtype, io, seed=dk)
+
+
 @pytest.mark.parametrize("cache_dtype,io", [(BF16, F32), (BF16, BF16), (F32, BF16), (F32, F32)])
 @pytest.mark.parametrize("heads,hk,page,dk,lens", [(4, 4, 16, 64, EDGE), (20, 5, 5, 128, [3000, 1, 0, 64, 65]), (32, 2, 64, 100, [500, 700]),
                                                    (8, 1, 16, 128, [6001])])
