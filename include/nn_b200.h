@@ -350,7 +350,8 @@ nnb_status nnb_paged_append(nnb_engine* e, const nnb_paged_cache* c, const nnb_p
  * (n_seq, n_head) f32 may be NULL.  scale = 0 stands for 1 / sqrt(dk).  A sequence without any position gets d_out = 0 and
  * d_lse = -inf; positions on a page outside the pool take no part.
  * accumulate != 0: also adds sum over the group's query heads of softmax(x)_t to the d_weight of every position.
- * Products and sums are held in f32 (bf16 operands enter exactly); d_ws is device memory of at least
+ * Products and sums are held in f32 (bf16 operands enter exactly; with bf16 queries on a bf16 cache the softmax's weights
+ * enter the product with V with 16 bits, half a step of the output being 2^-8); d_ws is device memory of at least
  * nnb_paged_attention_workspace bytes, 16-byte aligned, whose content need not be kept (0 from that call: invalid
  * arguments). */
 size_t nnb_paged_attention_workspace(nnb_engine* e, const nnb_paged_cache* c, const nnb_paged_seqs* s, size_t n_head, int accumulate);

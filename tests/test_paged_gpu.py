@@ -53,11 +53,13 @@ def _read(cache, table, seq, n):
 
 def _check_decode(cache, table, lens, q, out, lse, scale=None, w_before=None):
     """Bounds: a score is a dot product of dk terms, off by (dk + 4) u sum |q k| scale + its own rounding; p = exp(x - m) is off
-    by twice that (numerator and sum) plus a few u of exp; the sums over n positions by n u; all relative to sum p |v|."""
+    by twice that (numerator and sum) plus a few u of exp; the sums over n positions by n u; all relative to sum p |v|.
+    With bf16 queries on a bf16 cache p enters the product with V as two bf16 pieces: the leading 8 bits cut off leave less than
+    2^-7 p, whose rounding to 8 bits is off by at most half a step, 2^-8 of it: 2^-15 p in all."""
     hk, dk, heads = cache.n_head_kv, cache.dk, q.shape[1]
     g = heads // hk
     scale = dk ** -0.5 if scale is None else scale
-    half = HALF[out.dtype]
+    half, cut = HALF[out.dtype], 2.0 ** -15 if q.dtype == cache.k.dtype == BF16 else 0.0
     out, lse, q = out.cpu().double(), lse.cpu().double(), q.cpu().double()
     for i, n in enumerate(lens):
         if n == 0:
@@ -69,7 +71,7 @@ def _check_decode(cache, table, lens, q, out, lse, scale=None, w_before=None):
         delta = ((dk + 4) * U * abs(scale) * torch.einsum("hgd,htd->hgt", qq.abs(), k.abs())).amax(-1, keepdim=True) + 4 * U * x.abs().amax(-1, keepdim=True) + 8 * U
         p = torch.softmax(x, -1)
         want = torch.einsum("hgt,htd->hgd", p, v)
-        tol = (2 * delta + (n + 16) * U) * torch.einsum("hgt,htd->hgd", p, v.abs())
+        tol = (2 * delta + (n + 16) * U + cut) * torch.einsum("hgt,htd->hgd", p, v.abs())
         got = out[i].view(hk, g, dk)
         assert bool(((got - want).abs() <= tol + half * (want.abs() + tol) + 1e-38).all()), (i, n, ((got - want).abs() - tol).max())
         z = torch.logsumexp(x, -1)
