@@ -353,7 +353,7 @@ nnb_status nnb_paged_append(nnb_engine* e, const nnb_paged_cache* c, const nnb_p
  * Products and sums are held in f32 (bf16 operands enter exactly; with bf16 queries on a bf16 cache the softmax's weights
  * enter the product with V with 16 bits, half a step of the output being 2^-8); d_ws is device memory of at least
  * nnb_paged_attention_workspace bytes, 16-byte aligned, whose content need not be kept (0 from that call: invalid
- * arguments). */
+ * arguments); with accumulate it holds a score per query head and position of the table. */
 size_t nnb_paged_attention_workspace(nnb_engine* e, const nnb_paged_cache* c, const nnb_paged_seqs* s, size_t n_head, int accumulate);
 nnb_status nnb_paged_attention_decode(nnb_engine* e, const nnb_paged_cache* c, const nnb_paged_seqs* s, const void* d_q, int dtype,
                                       size_t q_stride, size_t n_head, float scale, void* d_out, float* d_lse, int accumulate, void* d_ws,
