@@ -123,7 +123,9 @@ __device__ __forceinline__ void advance_length(const PagedView& c, const SeqView
 // and each output written once; the asynchronous copies hide the chain of lookups (1.8 us) and angles (0.9 us), which with
 // loads into registers cost as much again as the features (8400 tokens of 20 + 2 x 5 heads of 128: 41 us).
 // Features that are not 16-byte aligned are loaded directly.
-constexpr int APPEND_TOKENS = 4;
+// (Room for eight tokens' angles although four are taken: what it leaves, five CTAs per SM, is better than six by 31 to 34 us
+// for the tokens above.)
+constexpr int APPEND_TOKENS = 8, APPEND_MANY = 4;
 constexpr size_t APPEND_SMEM = 64 * 1024;
 template <typename TI, typename TC, int VEC, bool STAGED>
 __global__ void __launch_bounds__(512) paged_append_kernel(const PagedView c, const SeqView s, const AppendArgs a, int tokens, int* flags)
@@ -269,7 +271,7 @@ static nnb_status launch_append(nnb_engine* e, const PagedView& c, const SeqView
     // Few tokens: one per CTA, a thread for every vector.  Many: four, whose lookups are done side by side (8400 tokens of 20 + 2 x 5
     // heads of 128 take 44 / 34 / 31 / 36 us with 1 / 2 / 4 / 8 per CTA of 256 threads).
     const bool few = n_rows <= 4 * (size_t)e->sm_count;
-    size_t tokens = few ? 1 : APPEND_TOKENS;
+    size_t tokens = few ? 1 : APPEND_MANY;
     if (staged && tokens > APPEND_SMEM / row) tokens = APPEND_SMEM / row;
     const unsigned threads = !few ? 256 : items >= 512 ? 512 : (unsigned)(items + 31) / 32 * 32;
     const bool lengths = a.row_start && a.len_out && a.len_out != s.len;
