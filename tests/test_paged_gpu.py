@@ -171,6 +171,34 @@ def test_decode_is_the_same_every_time_and_ignores_batch_neighbours(pkg, eng):
     _check_decode(cache, table[2:3], [2500], q[2:3], o, z)
 
 
+@pytest.mark.parametrize("cache_dtype", [F32, BF16])
+@pytest.mark.parametrize("lens", [[90, 0, 33], [3000, 5, 70]])
+def test_decode_through_the_c_interface_without_lse(pkg, eng, lens, cache_dtype):
+    """d_lse NULL with accumulated weights; a workspace full of NaN, exactly as large as asked for; one byte less is refused."""
+    import ctypes as C
+
+    lib = pkg.lib()
+    cache, table, lengths = _pool(pkg, eng, lens, 2, 16, 64, cache_dtype, track=True)
+    w0 = cache.weight.clone()
+    q = torch.randn((3, 8, 64), device=eng.device)
+    want, _ = eng.paged_attention_decode(cache, table, lengths, q, accumulate=True)
+    w1 = cache.weight.clone()
+    cache.weight.copy_(w0)
+    from neuralnet_cpp_b200 import paged
+
+    s = paged._Seqs(table.data_ptr(), lengths.data_ptr(), 3, table.shape[1], table.stride(0))
+    size = lib.nnb_paged_attention_workspace(eng.handle, C.byref(cache._c), C.byref(s), 8, 1)
+    ws = torch.full((size // 4 + 64,), float("nan"), device=eng.device)
+    out = torch.empty_like(q)
+    call = lambda n: lib.nnb_paged_attention_decode(eng.handle, C.byref(cache._c), C.byref(s), q.data_ptr(), 0, 512, 8, 0.0, out.data_ptr(), None, 1,  # noqa: E731
+                                                    ws.data_ptr(), n)
+    assert call(size - 1) == -1 and b"too small" in lib.nnb_last_error()
+    assert call(size) == 0
+    eng.check_device_errors()
+    assert torch.equal(out, want) and torch.equal(cache.weight.nan_to_num(9.0), w1.nan_to_num(9.0))
+    assert bool(ws[size // 4:].isnan().all())  # nothing behind the workspace was touched
+
+
 def test_sequences_may_share_pages(pkg, eng):
     """The completions of one prompt: their tables begin with the same pages."""
     cache, table, lengths, q, out, _ = _decode(pkg, eng, [256, 300, 280], 8, 2, 16, 64, BF16, F32, seed=9)
