@@ -242,6 +242,16 @@ def test_bad_pages_and_lengths_are_skipped_and_reported(pkg, eng, cache_dtype):
     eng.check_device_errors()
 
 
+def test_row_of_a_position(pkg, eng):
+    cache, table, lengths = _pool(pkg, eng, [40, 7], 3, 16, 100, BF16, track=True)
+    k, v, w = _read(cache, table, 0, 40)
+    rows = cache.k.view(-1, cache.pitch).cpu()
+    for head, pos in ((0, 0), (2, 15), (1, 16), (2, 39)):
+        r = cache.row(table[0].tolist(), head, pos)
+        assert torch.equal(rows[r, :100].double(), k[head, pos]) and cache.weight.view(-1)[r].item() == w[head, pos].item()
+    assert cache.row(table[0].tolist(), 0, 16 * table.shape[1]) == -1 and cache.row(table[1].tolist(), 0, 16) == -1
+
+
 def test_offsets_beyond_32_bits(pkg, eng):
     """A pool of more than 2^31 elements per tensor; the sequences' pages lie at its end."""
     hk, page, dk = 8, 64, 128
@@ -719,7 +729,8 @@ def test_a_serving_loop(pkg, eng, cache_dtype):
         pos += 1
 
 
-def test_captured_steps_follow_lengths_and_tables(pkg, eng):
+@pytest.mark.parametrize("cols", [1, 150])  # a short table (a cluster per item) and a long one (workers and a joining launch)
+def test_captured_steps_follow_lengths_and_tables(pkg, eng, cols):
     """append, decode (weights accumulated), evict and adjust_logits captured once on a side stream, replayed with other lengths,
     tables and inputs; two graphs captured from the same calls do not disturb each other."""
     n, heads, hk, dk, page = 4, 8, 2, 128, 16
@@ -729,7 +740,7 @@ def test_captured_steps_follow_lengths_and_tables(pkg, eng):
     side.wait_stream(torch.cuda.current_stream())
 
     def state(seed):
-        cache, table, lengths = _pool(pkg, eng, lens, hk, page, dk, BF16, seed=seed, room=64, track=True)
+        cache, table, lengths = _pool(pkg, eng, lens, hk, page, dk, BF16, seed=seed, room=64, track=True, extra_cols=cols)
         q, k, v = (torch.randn((n, h, dk), device=eng.device) for h in (heads, hk, hk))
         dst = pkg.PagedCache.empty(8, hk, page, dk, device=eng.device, track_weight=True)
         dt = torch.arange(8, dtype=torch.int32, device=eng.device).view(4, 2)
